@@ -72,7 +72,11 @@ typedef enum { KVF_INT4 = 0, KVF_INT8 = 1, KVF_F32 = 2 } kvf_data_type;
 typedef enum { KVF_PER_CHANNEL = 0, KVF_PER_TOKEN = 1 } kvf_quant_axis;
 /* element type of an input tensor; the reference takes f32 only
  * (crates/kvforge-python/src/py_types.rs:21-25); f16 is up-cast exactly. */
-typedef enum { KVF_IN_F32 = 0, KVF_IN_F16 = 1 } kvf_in_dtype;
+typedef enum {
+  KVF_IN_F32 = 0,
+  KVF_IN_F16 = 1,
+  KVF_IN_BF16 = 2 /* paged caches only: the codec's entry points refuse it */
+} kvf_in_dtype;
 /* CompressionPreset (crates/kvforge-core/src/pipeline.rs:5-15) */
 typedef enum {
   KVF_CONSERVATIVE = 0,
@@ -95,6 +99,7 @@ typedef struct {
 typedef struct kvf_ctx kvf_ctx;
 typedef struct kvf_basis kvf_basis;
 typedef struct kvf_compressed kvf_compressed;
+typedef struct kvf_paged_plan kvf_paged_plan;
 
 /* ---- context ---------------------------------------------------------- */
 /* replaces KernelLauncher::new (kernel_launcher.rs:13-17). Free every
@@ -393,6 +398,90 @@ kvf_status kvf_compressed_basis_bytes(const kvf_compressed* c, size_t* out);
 /* calibration scores of the keys (H floats, device), or NULL when calibration
  * was disabled or failed (the reference discards both, pipeline.rs:104-111) */
 const float* kvf_compressed_calibration(const kvf_compressed* c);
+
+/* ---- paged cache --------------------------------------------------------
+ * An uncompressed cache of many growing sequences, the attention of new tokens
+ * on it, the attention weight that every cached token has received, and
+ * eviction by that weight: what a serving program does with a layer before (or
+ * instead of) handing it to the codec. No counterpart in the reference.
+ *
+ * Slot j (0 <= j < kv_len) of a sequence lies in row j % page_size of page
+ * table[j / page_size]; the rows of one KV head of one page are contiguous. */
+typedef struct {
+  int32_t dtype;     /* kvf_in_dtype of keys, values, new rows, queries and outputs */
+  int32_t page_size; /* 16, 32, 64 or 128 */
+  size_t num_layers; /* layers stacked in the arrays below */
+  size_t num_pages;  /* pages of one layer */
+  size_t num_heads;  /* KV heads */
+  size_t head_dim;   /* 1..256 */
+  void* keys;        /* [num_layers, num_pages, num_heads, page_size, head_dim], device, 16-byte aligned */
+  void* values;      /* the same */
+  float* weights;    /* [num_layers, num_pages, num_heads, page_size], or NULL: no weights are kept */
+} kvf_paged_pool;
+
+/* A plan fixes what one step's calls on every layer share: sequence i has
+ * kv_lens_host[i] cached slots (its new tokens included) in the pages of row i
+ * of page_table_host (rows table_stride apart), and query_lens_host[i] new
+ * tokens, which are its last slots. Tokens of all sequences are numbered one
+ * after another, in the order of the sequences. query_heads is a multiple of
+ * the pool's num_heads (0: the plan is not for attention). A query at slot a
+ * sees slot j when j <= a and (window == 0 or j > a - window or j < sinks). A
+ * sequence may have more queries than slots: its first queries then lie before
+ * slot 0 and see nothing. Every page that the lengths reach is checked against
+ * num_pages; the arrays are read before the call returns. The plan copies them
+ * to the device on `stream` and may be used on any stream; on another one its
+ * calls first wait for that copy. kvf_paged_plan_free returns its memory after
+ * the last call issued with it on every stream; `stream` and the context must
+ * outlive it. */
+kvf_status kvf_paged_plan_create(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs,
+                                 const int32_t* query_lens_host, const int32_t* kv_lens_host,
+                                 const int32_t* page_table_host, size_t table_stride, size_t query_heads,
+                                 int32_t window, int32_t sinks, kvf_paged_plan** out, void* stream);
+kvf_status kvf_paged_plan_free(kvf_paged_plan* plan);
+
+/* Writes the plan's new tokens into one layer's pages: keys and values
+ * [tokens, num_heads, head_dim] with the given strides in elements (the last
+ * axis contiguous); their weights, where the pool keeps any, become 0. */
+kvf_status kvf_paged_append(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                            const void* keys, size_t k_token_stride, size_t k_head_stride, const void* values,
+                            size_t v_token_stride, size_t v_head_stride, void* stream);
+
+/* Copies one sequence of one layer out of its pages: keys and values
+ * [num_heads, kv_len, head_dim] of the pool's dtype, the codec's layout. */
+kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                            size_t seq, void* keys, void* values, void* stream);
+
+/* Attention of the plan's new tokens (already in the cache) over one layer:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j   over the slots j that t sees,
+ * query head h reading KV head h / (query_heads / num_heads). q [tokens,
+ * query_heads, head_dim] with strides in elements; out [tokens, query_heads,
+ * head_dim] contiguous, of the pool's dtype; lse (or NULL) f32 [tokens,
+ * query_heads], the natural logarithm of the softmax's sum. Scores, softmax
+ * and sums are held in f32; with f16 and bf16 pools the softmax's numerators
+ * are rounded to that type for the product with the values. A row that sees
+ * nothing, or only scores of -inf, gives out 0 and lse -inf. Slots that no row
+ * sees may hold anything, NaN included.
+ * decay < 0 leaves the weights alone; otherwise every slot of every sequence
+ * that has new tokens gets weight = decay * weight + sum over the new tokens
+ * and the KV head's query heads of the slot's softmax weight (decay 0
+ * overwrites). The sums run in a fixed order: results do not change from run
+ * to run. Stream-ordered; no host synchronisation. */
+kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                               const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
+                               float decay, void* out, float* lse, void* stream);
+
+/* Keeps `budget` slots of every sequence of the plan, for each layer and KV
+ * head on its own: the first `sinks`, the last `recent`, and of the others
+ * those with the largest weight (among equals the lowest slot; NaN counts
+ * below every number). The kept slots' keys, values and weights are copied, in
+ * order, into the pages of new_table_host [num_seqs, new_table_stride], which
+ * must be disjoint from the plan's; the sources stay as they are. A sequence
+ * of at most `budget` slots keeps them all. kept (device) [num_layers,
+ * num_seqs, num_heads, budget] i32: the slots, -1 behind the last.
+ * KVF_ERR_INVALID_CONFIG when sinks + recent > budget. */
+kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t budget,
+                           size_t recent, size_t sinks, const int32_t* new_table_host, size_t new_table_stride,
+                           int32_t* kept, void* stream);
 
 /* ---- cost model with measured GPU costs (CostModel, crates/kvforge-core/src/cost.rs;
  *      the reference's CpuCostModel is a fixed table, crates/kvforge-cpu/src/cost.rs:9-115)

@@ -25,7 +25,8 @@ __all__ = [
     "KVCache", "CompressedKV", "CompressionPipeline", "StreamingCompressor", "GpuCostModel", "BandwidthTier",
     "CostEstimate", "compress_adaptive", "compress", "decompress", "KvForgeError",
     "Basis", "QuantParams", "EntropyState", "GpuQuantizer", "GpuProjector", "GpuSensitivityCalibrator",
-    "GpuEntropyCodec", "config_from_preset", "parse_preset", "INT4", "INT8", "F32", "PER_CHANNEL", "PER_TOKEN",
+    "GpuEntropyCodec", "PagedKVCache", "PagedBatch", "Eviction", "config_from_preset", "parse_preset",
+    "INT4", "INT8", "F32", "PER_CHANNEL", "PER_TOKEN",
 ]
 
 INT4, INT8, F32 = L.INT4, L.INT8, L.F32
@@ -771,3 +772,7 @@ class GpuEntropyCodec:
         L.check(L.lib().kvf_rans_decode(L.context(dev), _ptr(d), d.numel(), _ptr(f), state.original_len, _ptr(out),
                                         _stream(dev)))
         return out
+
+
+# the paged cache in front of the codec
+from .paged import Eviction, PagedBatch, PagedKVCache  # noqa: E402

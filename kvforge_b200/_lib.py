@@ -33,7 +33,7 @@ STATUS_NAMES = {
 
 INT4, INT8, F32 = 0, 1, 2
 PER_CHANNEL, PER_TOKEN = 0, 1
-IN_F32, IN_F16 = 0, 1
+IN_F32, IN_F16, IN_BF16 = 0, 1, 2
 CONSERVATIVE, BALANCED, AGGRESSIVE, ADAPTIVE = 0, 1, 2, 3
 RECON_AUTO, RECON_CUDA_CORE, RECON_TENSOR_CORE = 0, 1, 2
 PROJ_AUTO, PROJ_CUDA_CORE, PROJ_TENSOR_CORE, PROJ_TENSOR_CORE_APPROX = 0, 1, 2, 3
@@ -56,6 +56,8 @@ EXPORTS = [
     "kvf_bandwidth_bytes_per_us", "kvf_cost_measure", "kvf_cost_estimate", "kvf_cost_select",
     "kvf_launch_count", "kvf_stage_name", "kvf_profile_enable", "kvf_profile_read", "kvf_calibrate_noalloc",
     "kvf_set_projection_engine", "kvf_compress_layers", "kvf_compressed_free_many",
+    "kvf_paged_plan_create", "kvf_paged_plan_free", "kvf_paged_append", "kvf_paged_gather", "kvf_paged_attention",
+    "kvf_paged_evict",
 ]
 
 NUM_STAGES = 8
@@ -73,6 +75,21 @@ class PipelineConfig(C.Structure):
         ("projection_variance_threshold", C.c_double),
         ("enable_entropy_coding", C.c_int32),
         ("enable_calibration", C.c_int32),
+    ]
+
+
+class PagedPool(C.Structure):
+    """kvf_paged_pool: the arrays of a paged cache."""
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("page_size", C.c_int32),
+        ("num_layers", C.c_size_t),
+        ("num_pages", C.c_size_t),
+        ("num_heads", C.c_size_t),
+        ("head_dim", C.c_size_t),
+        ("keys", C.c_void_p),
+        ("values", C.c_void_p),
+        ("weights", C.c_void_p),
     ]
 
 
@@ -171,6 +188,12 @@ def _declare(L):
         "kvf_cost_estimate": (st, [C.POINTER(PresetCost), sz, sz, i32, C.c_double, C.POINTER(CostEstimate)]),
         "kvf_cost_select": (st, [C.POINTER(PresetCost), sz, sz, C.c_double, C.c_double, C.POINTER(CostEstimate),
                                  szp]),
+        "kvf_paged_plan_create": (st, [p, C.POINTER(PagedPool), sz, p, p, p, sz, sz, i32, i32, C.POINTER(p), p]),
+        "kvf_paged_plan_free": (st, [p]),
+        "kvf_paged_append": (st, [p, p, C.POINTER(PagedPool), sz, p, sz, sz, p, sz, sz, p]),
+        "kvf_paged_gather": (st, [p, p, C.POINTER(PagedPool), sz, sz, p, p, p]),
+        "kvf_paged_attention": (st, [p, p, C.POINTER(PagedPool), sz, p, sz, sz, C.c_float, C.c_float, p, p, p]),
+        "kvf_paged_evict": (st, [p, p, C.POINTER(PagedPool), sz, sz, sz, p, sz, p, p]),
         "kvf_launch_count": (C.c_uint64, []),
         "kvf_stage_name": (C.c_char_p, [i32]),
         "kvf_profile_enable": (st, [p, C.c_int]),

@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "kvf_internal.cuh"
+#include "kvf_paged.cuh"
 
 using namespace kvf;
 
@@ -219,6 +220,35 @@ struct kvf_ctx {
     std::lock_guard<std::mutex> lock(mu);
     order_spare.push_back(e);
   }
+  // pinned host buffers that stage a paged plan's tables, reused across plans;
+  // `done` is recorded behind the copy out of a buffer
+  struct Pinned {
+    void* p = nullptr;
+    size_t cap = 0;
+    cudaEvent_t done = nullptr;
+  };
+  std::vector<Pinned> pinned_spare;
+  cudaError_t pinned(size_t bytes, Pinned* out) {
+    {
+      std::lock_guard<std::mutex> lock(mu);
+      for (size_t i = 0; i < pinned_spare.size(); ++i)
+        if (pinned_spare[i].cap >= bytes && cudaEventQuery(pinned_spare[i].done) == cudaSuccess) {
+          *out = pinned_spare[i];
+          pinned_spare.erase(pinned_spare.begin() + i);
+          return cudaSuccess;
+        }
+    }
+    Pinned b;
+    b.cap = std::max<size_t>(4096, bytes + bytes / 2);
+    cudaError_t e = cudaEventCreateWithFlags(&b.done, cudaEventDisableTiming);
+    if (e == cudaSuccess && (e = cudaMallocHost(&b.p, b.cap)) != cudaSuccess) cudaEventDestroy(b.done);
+    if (e == cudaSuccess) *out = b;
+    return e;
+  }
+  void pinned_release(const Pinned& b) {
+    std::lock_guard<std::mutex> lock(mu);
+    pinned_spare.push_back(b);
+  }
   cudaEvent_t event() {
     std::lock_guard<std::mutex> lock(mu);
     if (!spare.empty()) {
@@ -344,14 +374,16 @@ kvf_status check_shape(size_t H, size_t T, size_t D) {
   return KVF_OK;
 }
 
-// a reader of `c` on stream `st`: waits for the object's buffers to be
-// complete when `st` is not the stream that built them
-kvf_status reader_enter(const kvf_compressed* c, cudaStream_t st) {
+// a reader of `c` (a compressed layer, a paged plan) on stream `st`: waits for
+// the object's buffers to be complete when `st` is not the stream that built them
+template <class Obj>
+kvf_status reader_enter(const Obj* c, cudaStream_t st) {
   if (c->ready && st != c->stream) KVF_CUDA(cudaStreamWaitEvent(st, c->ready, 0));
   return KVF_OK;
 }
-// ... and after its last use: records on `st` what kvf_compressed_free waits for
-kvf_status reader_leave(const kvf_compressed* c, cudaStream_t st) {
+// ... and after its last use: records on `st` what the object's free waits for
+template <class Obj>
+kvf_status reader_leave(const Obj* c, cudaStream_t st) {
   if (st == c->stream) return KVF_OK;
   std::lock_guard<std::mutex> lock(c->use_mu);
   cudaEvent_t ev = nullptr;
@@ -951,6 +983,196 @@ kvf_status read_status(kvf_ctx* ctx, cudaStream_t st) {
 }  // namespace
 
 // =============================================================================
+// ---- paged cache ----------------------------------------------------------------
+struct kvf_paged_plan {
+  kvf_ctx* ctx = nullptr;
+  int device = 0;
+  cudaStream_t stream = nullptr;
+  // what the pool must be like
+  int dtype = 0, page_size = 0;
+  size_t num_pages = 0, heads = 0, dim = 0;
+  size_t tokens = 0, group = 0;
+  int window = 0, sinks = 0;
+  std::vector<int> kv_lens, q_lens, pages;  // pages: every page in use, sequence after sequence
+  std::vector<size_t> page_start;           // [n + 1] into pages
+  void* block = nullptr;  // device: tables and work lists
+  PagedSeqs seqs;
+  std::vector<PagedWork> works;
+  const PagedSlots* slots = nullptr;  // tiles of slots whose weights change
+  size_t slots_n = 0;
+  bool few_rows = false;  // every sequence has at most kGenRowsShort rows per KV head
+  cudaEvent_t ready = nullptr;
+  mutable std::mutex use_mu;
+  mutable std::vector<std::pair<cudaStream_t, cudaEvent_t>> uses;
+};
+
+namespace {
+
+constexpr size_t kMaxLen = size_t(1) << 30;  // slots of a sequence, tokens of a plan
+
+kvf_status check_pool(const kvf_paged_pool* pool) {
+  if (!pool) return fail(KVF_ERR_INVALID_CONFIG, "null pool");
+  if (pool->dtype != KVF_IN_F32 && pool->dtype != KVF_IN_F16 && pool->dtype != KVF_IN_BF16)
+    return fail(KVF_ERR_INVALID_CONFIG, "unknown pool dtype");
+  if (pool->page_size != 16 && pool->page_size != 32 && pool->page_size != 64 && pool->page_size != 128)
+    return fail(KVF_ERR_INVALID_CONFIG, "page_size must be 16, 32, 64 or 128");
+  if (pool->head_dim == 0 || pool->head_dim > 256) return fail(KVF_ERR_SHAPE_MISMATCH, "head_dim must be in 1..256");
+  if (pool->num_heads == 0 || pool->num_heads > 65535)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "num_heads must be in 1..65535");
+  if (pool->num_layers == 0 || pool->num_layers > 65535)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "num_layers must be in 1..65535");
+  if (pool->num_pages == 0 || pool->num_pages > 0x7fffffffu / pool->num_heads)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "num_pages * num_heads must be in 1..2^31-1");
+  if (!pool->keys || !pool->values) return fail(KVF_ERR_INVALID_CONFIG, "null pool pointer");
+  if (!aligned(pool->keys, 16) || !aligned(pool->values, 16) || !aligned(pool->weights, 4))
+    return fail(KVF_ERR_INVALID_CONFIG, "pool arrays must be 16-byte aligned");
+  return KVF_OK;
+}
+
+kvf_status check_plan(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer) {
+  KVF_TRY(check_ctx(ctx));
+  if (!plan) return fail(KVF_ERR_INVALID_CONFIG, "null plan");
+  KVF_TRY(check_pool(pool));
+  if (plan->ctx != ctx) return fail(KVF_ERR_INVALID_CONFIG, "the plan belongs to another context");
+  if (plan->dtype != pool->dtype || plan->page_size != pool->page_size || plan->num_pages != pool->num_pages ||
+      plan->heads != pool->num_heads || plan->dim != pool->head_dim)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "the plan was made for another pool");
+  if (layer >= pool->num_layers) return fail(KVF_ERR_SHAPE_MISMATCH, "layer outside the pool");
+  return KVF_OK;
+}
+
+PagedLayer paged_layer(const kvf_paged_pool* pool, size_t layer) {
+  PagedLayer c;
+  c.dtype = pool->dtype;
+  while ((1 << c.page_shift) < pool->page_size) ++c.page_shift;
+  c.pages = (int)pool->num_pages;
+  c.heads = (int)pool->num_heads;
+  c.dim = (int)pool->head_dim;
+  const size_t rows = layer * pool->num_pages * pool->num_heads * pool->page_size;
+  const size_t e = pool->dtype == KVF_IN_F32 ? 4 : 2;
+  c.keys = static_cast<char*>(pool->keys) + rows * pool->head_dim * e;
+  c.values = static_cast<char*>(pool->values) + rows * pool->head_dim * e;
+  c.weights = pool->weights ? pool->weights + rows : nullptr;
+  return c;
+}
+
+// host image of a device block of arrays, each 16-byte aligned
+struct BlockImage {
+  std::vector<char> bytes;
+  template <class T>
+  size_t add(const T* p, size_t n) {
+    const size_t at = bytes.size();
+    bytes.resize(align_up(at + n * sizeof(T), 16));
+    if (n) std::memcpy(bytes.data() + at, p, n * sizeof(T));
+    return at;
+  }
+  template <class T>
+  size_t add(const std::vector<T>& v) {
+    return add(v.data(), v.size());
+  }
+};
+
+// `bytes` host bytes to the device, through a pinned buffer, without waiting
+kvf_status upload(kvf_ctx* ctx, void* dst, const void* src, size_t bytes, cudaStream_t st) {
+  kvf_ctx::Pinned pin;
+  KVF_CUDA(ctx->pinned(bytes, &pin));
+  std::memcpy(pin.p, src, bytes);
+  cudaError_t e = cudaMemcpyAsync(dst, pin.p, bytes, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess) e = cudaEventRecord(pin.done, st);
+  ctx->pinned_release(pin);
+  KVF_CUDA(e);
+  return KVF_OK;
+}
+
+kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, const int32_t* kv_lens,
+                           const int32_t* table, size_t stride, size_t query_heads) {
+  size_t tokens = 0, max_pages = 1, max_kv = 0;
+  p->page_start.assign(1, 0);
+  for (size_t i = 0; i < n; ++i) {
+    if (q_lens[i] < 0 || kv_lens[i] < 0 || (size_t)kv_lens[i] > kMaxLen || (size_t)q_lens[i] > kMaxLen)
+      return fail(KVF_ERR_SHAPE_MISMATCH, "sequence lengths must be in 0..2^30");
+    tokens += (size_t)q_lens[i];
+    max_kv = std::max(max_kv, (size_t)kv_lens[i]);
+    const size_t pages = ((size_t)kv_lens[i] + p->page_size - 1) / p->page_size;
+    if (pages > stride) return fail(KVF_ERR_SHAPE_MISMATCH, "page table shorter than a sequence");
+    for (size_t k = 0; k < pages; ++k) {
+      const int32_t id = table[i * stride + k];
+      if (id < 0 || (size_t)id >= p->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
+      p->pages.push_back(id);
+    }
+    p->page_start.push_back(p->pages.size());
+    max_pages = std::max(max_pages, pages);
+  }
+  if (tokens > kMaxLen) return fail(KVF_ERR_SHAPE_MISMATCH, "more than 2^30 new tokens");
+  if (tokens * p->group > kMaxLen) return fail(KVF_ERR_SHAPE_MISMATCH, "more than 2^30 query rows per KV head");
+  p->tokens = tokens;
+  p->kv_lens.assign(kv_lens, kv_lens + n);
+  p->q_lens.assign(q_lens, q_lens + n);
+  // a window or sinks that reach over every slot hide nothing
+  if ((size_t)p->window >= max_kv || (size_t)p->sinks >= max_kv) p->window = p->sinks = 0;
+
+  BlockImage img;
+  std::vector<int> tab(n * max_pages, 0), q_start(n + 1, 0);
+  for (size_t i = 0; i < n; ++i) {
+    std::copy(p->pages.begin() + p->page_start[i], p->pages.begin() + p->page_start[i + 1],
+              tab.begin() + i * max_pages);
+    q_start[i + 1] = q_start[i] + q_lens[i];
+  }
+  const size_t at_table = img.add(tab), at_kv = img.add(p->kv_lens), at_q = img.add(q_start);
+
+  struct Offsets { size_t segs, first, joins; };
+  std::vector<Offsets> at;
+  std::vector<PagedWorkHost> hosts;
+  std::vector<PagedSlots> slots;
+  if (query_heads && tokens) {
+    int sms = 0;
+    KVF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device));
+    const int group = (int)p->group, heads = (int)p->heads;
+    hosts.resize(2);
+    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, kGenRowsShort, kGenRowsShort, kGenKeys,
+                3 * sms, 2, 1, &hosts[0]);
+    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, kGenRowsShort + 1, (long long)kMaxLen, kGenRows,
+                kGenKeys, 2 * sms, 2, 1, &hosts[1]);
+    p->few_rows = hosts[1].segs.empty();
+    for (size_t i = 0; i < n; ++i)
+      if (q_lens[i])
+        for (int j = 0; j < kv_lens[i]; j += kGenKeys) slots.push_back({(int)i, j});
+    for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});
+  }
+  const size_t at_slots = img.add(slots);
+
+  KVF_CUDA(cudaMallocFromPoolAsync(&p->block, img.bytes.size(), p->ctx->pool, p->stream));
+  KVF_TRY(upload(p->ctx, p->block, img.bytes.data(), img.bytes.size(), p->stream));
+  char* d = static_cast<char*>(p->block);
+  p->seqs.table = reinterpret_cast<const int*>(d + at_table);
+  p->seqs.stride = max_pages;
+  p->seqs.kv_len = reinterpret_cast<const int*>(d + at_kv);
+  p->seqs.q_start = reinterpret_cast<const int*>(d + at_q);
+  p->seqs.n = (int)n;
+  for (size_t i = 0; i < hosts.size(); ++i) {
+    const PagedWorkHost& h = hosts[i];
+    if (h.segs.empty()) continue;
+    PagedWork w;
+    w.row_tile = h.row_tile;
+    w.key_tile = h.key_tile;
+    w.ctas = (int)h.first.size() - 1;
+    w.segs_n = (int)h.segs.size();
+    w.joins_n = (int)h.joins.size();
+    w.parts = h.parts;
+    w.segs = reinterpret_cast<const PagedSeg*>(d + at[i].segs);
+    w.first = reinterpret_cast<const int*>(d + at[i].first);
+    w.joins = reinterpret_cast<const PagedJoin*>(d + at[i].joins);
+    p->works.push_back(w);
+  }
+  p->slots = reinterpret_cast<const PagedSlots*>(d + at_slots);
+  p->slots_n = slots.size();
+  KVF_CUDA(p->ctx->order_event(&p->ready));
+  KVF_CUDA(cudaEventRecord(p->ready, p->stream));
+  return KVF_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int kvf_abi_version(void) { return KVF_ABI_VERSION; }
@@ -997,6 +1219,11 @@ kvf_status kvf_destroy(kvf_ctx* ctx) {
   }
   for (auto e : ctx->spare) cudaEventDestroy(e);
   for (auto e : ctx->order_spare) cudaEventDestroy(e);
+  for (auto& b : ctx->pinned_spare) {
+    cudaEventSynchronize(b.done);  // its last copy
+    cudaEventDestroy(b.done);
+    cudaFreeHost(b.p);
+  }
   for (auto& kv : ctx->sides) {
     cudaStreamSynchronize(kv.second.s);
     cudaStreamDestroy(kv.second.s);
@@ -2122,6 +2349,200 @@ kvf_status kvf_cost_measure(kvf_ctx* ctx, const void* keys, const void* values, 
   for (int i = 0; i < 2; ++i)
     if (dout[i]) cudaFree(dout[i]);
   return s;
+}
+
+// ---- paged cache ----------------------------------------------------------------
+kvf_status kvf_paged_plan_create(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs,
+                                 const int32_t* query_lens_host, const int32_t* kv_lens_host,
+                                 const int32_t* page_table_host, size_t table_stride, size_t query_heads,
+                                 int32_t window, int32_t sinks, kvf_paged_plan** out, void* stream) {
+  KVF_TRY(check_ctx(ctx));
+  KVF_TRY(check_pool(pool));
+  if (!out) return fail(KVF_ERR_INVALID_CONFIG, "null output pointer");
+  if (num_seqs && (!query_lens_host || !kv_lens_host || (table_stride && !page_table_host)))
+    return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  if (num_seqs * pool->num_heads > 65535 || num_seqs > 65535)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "num_seqs * num_heads > 65535 is not supported");
+  if (query_heads % pool->num_heads)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "query_heads must be a multiple of the pool's num_heads");
+  if (query_heads > 65535) return fail(KVF_ERR_SHAPE_MISMATCH, "query_heads > 65535 is not supported");
+  if (window < 0 || sinks < 0) return fail(KVF_ERR_INVALID_CONFIG, "window and sinks must not be negative");
+  DeviceGuard g(ctx->device);
+  kvf_paged_plan* p = nullptr;
+  kvf_status s;
+  try {  // no exception leaves the C ABI
+    p = new kvf_paged_plan();
+    p->ctx = ctx;
+    p->device = ctx->device;
+    p->stream = S(stream);
+    p->dtype = pool->dtype;
+    p->page_size = pool->page_size;
+    p->num_pages = pool->num_pages;
+    p->heads = pool->num_heads;
+    p->dim = pool->head_dim;
+    p->group = query_heads / pool->num_heads;
+    p->window = window;
+    p->sinks = window ? sinks : 0;
+    s = paged_plan_body(p, num_seqs, query_lens_host, kv_lens_host, page_table_host, table_stride, query_heads);
+  } catch (const std::exception& ex) {
+    s = fail(KVF_ERR_PIPELINE, std::string("paged plan: ") + ex.what());
+  }
+  if (s != KVF_OK) {
+    const std::string msg = g_err;
+    kvf_paged_plan_free(p);
+    g_err = msg;
+    return s;
+  }
+  *out = p;
+  return KVF_OK;
+}
+
+kvf_status kvf_paged_plan_free(kvf_paged_plan* plan) {
+  if (!plan) return KVF_OK;
+  {
+    DeviceGuard g(plan->device);
+    for (auto& u : plan->uses) {
+      cudaStreamWaitEvent(plan->stream, u.second, 0);
+      plan->ctx->order_event_release(u.second);
+    }
+    if (plan->ready) plan->ctx->order_event_release(plan->ready);
+    if (plan->block) cudaFreeAsync(plan->block, plan->stream);
+  }
+  delete plan;
+  return KVF_OK;
+}
+
+kvf_status kvf_paged_append(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                            const void* keys, size_t k_token_stride, size_t k_head_stride, const void* values,
+                            size_t v_token_stride, size_t v_head_stride, void* stream) {
+  KVF_TRY(check_plan(ctx, plan, pool, layer));
+  if (plan->tokens == 0) return KVF_OK;
+  if (!keys || !values) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  const size_t e = plan->dtype == KVF_IN_F32 ? 4 : 2;
+  if (!aligned(keys, e) || !aligned(values, e)) return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
+  DeviceGuard g(ctx->device);
+  cudaStream_t st = S(stream);
+  KVF_TRY(reader_enter(plan, st));
+  KVF_CUDA(launch_paged_append(plan->seqs, paged_layer(pool, layer), plan->tokens, keys, k_token_stride, k_head_stride,
+                               values, v_token_stride, v_head_stride, st));
+  return reader_leave(plan, st);
+}
+
+kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                            size_t seq, void* keys, void* values, void* stream) {
+  KVF_TRY(check_plan(ctx, plan, pool, layer));
+  if (seq >= plan->kv_lens.size()) return fail(KVF_ERR_SHAPE_MISMATCH, "sequence outside the plan");
+  const size_t len = (size_t)plan->kv_lens[seq];
+  if (len == 0) return KVF_OK;
+  if (!keys || !values) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  const size_t e = plan->dtype == KVF_IN_F32 ? 4 : 2;
+  if (!aligned(keys, e) || !aligned(values, e)) return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
+  DeviceGuard g(ctx->device);
+  cudaStream_t st = S(stream);
+  KVF_TRY(reader_enter(plan, st));
+  KVF_CUDA(launch_paged_gather(plan->seqs, paged_layer(pool, layer), seq, len, keys, values, st));
+  return reader_leave(plan, st);
+}
+
+kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
+                               const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
+                               float decay, void* out, float* lse, void* stream) {
+  KVF_TRY(check_plan(ctx, plan, pool, layer));
+  if (plan->group == 0) return fail(KVF_ERR_INVALID_CONFIG, "the plan was made without query heads");
+  if (!std::isfinite(scale)) return fail(KVF_ERR_INVALID_CONFIG, "scale must be finite");
+  if (!(decay <= 1.0f)) return fail(KVF_ERR_INVALID_CONFIG, "decay must be at most 1");
+  if (decay >= 0.0f && !pool->weights) return fail(KVF_ERR_INVALID_CONFIG, "the pool keeps no weights");
+  if (plan->tokens == 0) return KVF_OK;
+  if (!query || !out) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  const size_t e = plan->dtype == KVF_IN_F32 ? 4 : 2;
+  if (!aligned(query, e) || !aligned(out, e) || !aligned(lse, 4))
+    return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
+  DeviceGuard g(ctx->device);
+  cudaStream_t st = S(stream);
+  Scratch sc(st, ctx->pool);
+  PagedAttn a;
+  a.s = plan->seqs;
+  a.c = paged_layer(pool, layer);
+  a.group = (int)plan->group;
+  a.window = plan->window;
+  a.sinks = plan->sinks;
+  a.q = query;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.scale2 = scale * 1.44269504088896340736f;
+  a.out = out;
+  a.lse = lse;
+  a.status = ctx->d_status;
+  if (decay >= 0.0f && !lse) {
+    a.lse = sc.get<float>(plan->tokens * plan->heads * plan->group);
+    if (!a.lse) return fail(KVF_ERR_CUDA, "scratch allocation failed");
+  }
+  KVF_TRY(reader_enter(plan, st));
+  cudaError_t err = cudaSuccess;
+  for (const PagedWork& w : plan->works) {
+    if (w.parts) {
+      const size_t rows = (size_t)w.parts * w.row_tile;
+      a.part_o = sc.get<float>(rows * plan->dim);
+      a.part_ml = sc.get<float>(rows * 2);
+      if (!a.part_o || !a.part_ml) err = cudaErrorMemoryAllocation;
+    }
+    if (err == cudaSuccess) err = launch_paged_attn_generic(a, w, st);
+    if (err == cudaSuccess) err = launch_paged_join(a, w, st);
+  }
+  if (err == cudaSuccess && decay >= 0.0f)
+    err = launch_paged_weights_generic(a, plan->slots, plan->slots_n, plan->few_rows, decay, st);
+  const kvf_status ls = reader_leave(plan, st);
+  KVF_CUDA(err);
+  return ls;
+}
+
+kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t budget,
+                           size_t recent, size_t sinks, const int32_t* new_table_host, size_t new_table_stride,
+                           int32_t* kept, void* stream) {
+  KVF_TRY(check_plan(ctx, plan, pool, 0));
+  if (!pool->weights) return fail(KVF_ERR_INVALID_CONFIG, "the pool keeps no weights");
+  if (budget == 0 || budget > kMaxLen) return fail(KVF_ERR_INVALID_CONFIG, "budget must be in 1..2^30");
+  if (recent > budget || sinks > budget - recent)
+    return fail(KVF_ERR_INVALID_CONFIG, "sinks and recent slots exceed the budget");
+  const size_t n = plan->kv_lens.size();
+  if (n == 0) return KVF_OK;
+  if (!new_table_host || !kept) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  DeviceGuard g(ctx->device);
+  cudaStream_t st = S(stream);
+  Scratch sc(st, ctx->pool);
+  int* table = nullptr;
+  size_t stride = 1;
+  try {  // no exception leaves the C ABI
+    std::vector<bool> used(plan->num_pages, false);
+    for (const int id : plan->pages) used[id] = true;
+    std::vector<size_t> count(n);
+    for (size_t i = 0; i < n; ++i) {
+      const size_t m = std::min(budget, (size_t)plan->kv_lens[i]);
+      count[i] = (m + plan->page_size - 1) / plan->page_size;
+      if (count[i] > new_table_stride) return fail(KVF_ERR_SHAPE_MISMATCH, "page table shorter than the budget");
+      stride = std::max(stride, count[i]);
+    }
+    std::vector<int> host(n * stride, 0);
+    for (size_t i = 0; i < n; ++i)
+      for (size_t k = 0; k < count[i]; ++k) {
+        const int32_t id = new_table_host[i * new_table_stride + k];
+        if (id < 0 || (size_t)id >= plan->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
+        if (used[id]) return fail(KVF_ERR_INVALID_CONFIG, "a new page is in use");
+        used[id] = true;
+        host[i * stride + k] = id;
+      }
+    table = sc.get<int>(host.size());
+    if (!table) return fail(KVF_ERR_CUDA, "scratch allocation failed");
+    KVF_TRY(upload(ctx, table, host.data(), host.size() * sizeof(int), st));
+  } catch (const std::exception& ex) {
+    return fail(KVF_ERR_PIPELINE, std::string("paged eviction: ") + ex.what());
+  }
+  KVF_TRY(reader_enter(plan, st));
+  const cudaError_t err = launch_paged_evict(plan->seqs, paged_layer(pool, 0), pool->num_layers, budget, recent, sinks,
+                                             table, stride, kept, st);
+  const kvf_status ls = reader_leave(plan, st);
+  KVF_CUDA(err);
+  return ls;
 }
 
 }  // extern "C"

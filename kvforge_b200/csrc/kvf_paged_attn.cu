@@ -1,0 +1,458 @@
+// Attention over a paged cache on CUDA cores (every type, head_dim up to 256),
+// the joining of cut tiles, and the attention weights of cached slots.
+//
+// One pass over the slots with the running maximum m and sum l of the softmax
+// (base 2: s2 = scale * log2(e) * q.k):
+//   m' = max(m, max s2);  f = 2^(m - m');  l' = f l + sum 2^(s2 - m');
+//   O' = f O + sum 2^(s2 - m') v
+// and out = O / l, lse = (m + log2 l) ln 2. A segment of the slots leaves
+// (m, l, O); k_paged_join adds segments up with the weights 2^(m_i - max m).
+// These kernels serve f32 pools, whose products need all 24 bits, and head
+// dims that the tensor-core kernels do not take.
+#include <cfloat>
+#include <cmath>
+
+#include "kvf_paged.cuh"
+
+namespace kvf {
+namespace {
+
+constexpr int kGenThreads = 256;
+constexpr int kPStride = kGenKeys + 4;  // rows of P, 16-byte aligned, four banks apart
+
+// element (r, c) of a tile of f32 rows in shared memory, rows of DP floats (a
+// multiple of 32): 16-byte groups are permuted by the row so that eight rows
+// at one column lie in different banks
+__device__ __forceinline__ int tile_at(int r, int c4, int DP) { return r * DP + ((c4 ^ (r & 7)) << 2); }
+
+// four (f32) or eight (16-bit) elements of a row as floats
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) x[i] = to_float(e[i]);
+}
+
+// Fills `rows` rows of DP floats; row(r) points at row r's first element, or
+// is nullptr for a row of zeros.
+template <typename T, typename Row>
+__device__ __forceinline__ void fill_tile(float* sm, int rows, int DP, int D, bool wide, Row row) {
+  if (wide) {
+    constexpr int E = 16 / sizeof(T);
+    const int per = DP / E;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * per; i += kGenThreads) {
+      const int r = i / per, c = (i - r * per) * E;
+      const T* p = row(r);
+      float x[E];
+      if (p && c < D) load16(p + c, x);
+      else
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(sm + tile_at(r, (c + e) >> 2, DP)) =
+            make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * DP; i += kGenThreads) {
+      const int r = i / DP, c = i - r * DP;
+      const T* p = row(r);
+      sm[tile_at(r, c >> 2, DP) + (c & 3)] = (p && c < D) ? to_float(p[c]) : 0.0f;
+    }
+  }
+}
+
+// scores of RT rows (ty * RT + i) and four slots (tx + 16 u) of this thread
+template <int RT>
+__device__ __forceinline__ void scores(const float* Q, const float* K, int DP, int ty, int tx, float (&s)[RT][4]) {
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[i][u] = 0.0f;
+#pragma unroll 2
+  for (int c = 0; c < DP / 4; ++c) {
+    float4 q[RT], k[4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) q[i] = *reinterpret_cast<const float4*>(Q + tile_at(ty * RT + i, c, DP));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u] = *reinterpret_cast<const float4*>(K + tile_at(tx + 16 * u, c, DP));
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s[i][u] = fmaf(q[i].x, k[u].x, s[i][u]);
+        s[i][u] = fmaf(q[i].y, k[u].y, s[i][u]);
+        s[i][u] = fmaf(q[i].z, k[u].z, s[i][u]);
+        s[i][u] = fmaf(q[i].w, k[u].w, s[i][u]);
+      }
+  }
+}
+
+// 16 lanes share a row
+__device__ __forceinline__ float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// A 16 x 16 arrangement of threads: thread (ty, tx) holds the scores of RT
+// rows and four slots, then those rows' sums of NU groups of four columns.
+// Tiles of 64 slots; 64 rows (RT = 4) where there are many, 16 (RT = 1) for
+// single tokens. Bound by the CUDA cores' multiply-adds at 64 rows and by
+// loads at 16, where two or three CTAs share an SM so that one loads while
+// another computes.
+template <typename T, int RT, int NU>
+__global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const PagedSeg* __restrict__ segs,
+                                                            const int* __restrict__ first, int DP, bool wide,
+                                                            bool wide_q) {
+  constexpr int BR = 16 * RT;
+  extern __shared__ float4 sm4[];
+  float* Q = reinterpret_cast<float*>(sm4);  // [BR][DP]
+  float* K = Q + BR * DP;                    // [64][DP]
+  float* V = K + kGenKeys * DP;              // [64][DP]
+  float* P = V + kGenKeys * DP;              // [BR][kPStride]
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int D = a.c.dim, Hq = a.c.heads * a.group;
+  const int s1 = __ldg(first + blockIdx.x + 1);
+  for (int si = __ldg(first + blockIdx.x); si < s1; ++si) {
+    const PagedSeg g = segs[si];
+    const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+    const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = min(BR, nq * a.group - g.row0);
+    const int* table = a.s.table + (size_t)g.seq * a.s.stride;
+    const PagedSpan span = paged_span(g.row0, BR, a.group, n, nq, a.window, a.sinks, kGenKeys);
+    __syncthreads();  // the previous segment's tiles are read
+    fill_tile<T>(Q, BR, DP, D, wide_q, [&](int r) -> const T* {
+      if (r >= rows) return nullptr;
+      const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+      return static_cast<const T*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
+    });
+    int pos[RT];
+    float m[RT], l[RT], o[RT][NU][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      pos[i] = n - nq + (g.row0 + ty * RT + i) / a.group;
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][u][e] = 0.0f;
+    }
+    const int pa = n - nq + g.row0 / a.group, pb = n - nq + (g.row0 + rows - 1) / a.group;
+    for (int it = g.it0; it < g.it1; ++it) {
+      const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kGenKeys;
+      __syncthreads();
+      // slots that no row of the tile sees (past the last one, between the
+      // sinks and the window) are zeros here, whatever their pages hold
+      auto slot = [&](const void* pool, int r) -> const T* {
+        const int j = j0 + r;
+        if (j > pb || (a.window && j <= pa - a.window && j >= a.sinks)) return nullptr;
+        return static_cast<const T*>(pool) + paged_row(table, a.c, g.head, j);
+      };
+      fill_tile<T>(K, kGenKeys, DP, D, wide, [&](int r) { return slot(a.c.keys, r); });
+      fill_tile<T>(V, kGenKeys, DP, D, wide, [&](int r) { return slot(a.c.values, r); });
+      __syncthreads();
+      float s[RT][4];
+      scores<RT>(Q, K, DP, ty, tx, s);
+      // a tile that every row sees whole needs no masks
+      const bool whole = j0 + kGenKeys - 1 <= pa &&
+                         (!a.window || j0 > pb - a.window || j0 + kGenKeys <= a.sinks);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float mx = m[i];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          s[i][u] *= a.scale2;
+          if (!whole && !paged_sees(pos[i], j0 + tx + 16 * u, a.window, a.sinks)) s[i][u] = -INFINITY;
+          mx = fmaxf(mx, s[i][u]);
+        }
+        mx = half_max(mx);
+        const float mu = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: all terms are 0
+        const float f = exp2f(m[i] - mu);
+        m[i] = mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float p = exp2f(s[i][u] - mu);
+          sum += p;
+          // a slot that the row does not see is marked, so that its value
+          // (infinite, or NaN) is skipped instead of multiplied by 0
+          const bool see = whole || paged_sees(pos[i], j0 + tx + 16 * u, a.window, a.sinks);
+          P[(ty * RT + i) * kPStride + tx + 16 * u] = see ? p : -1.0f;
+        }
+        l[i] = l[i] * f + half_sum(sum);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][u][e] *= f;
+      }
+      __syncwarp();  // the rows of P that this half-warp wrote are its own
+      auto accumulate = [&](auto masked) {
+#pragma unroll 1
+        for (int k4 = 0; k4 < kGenKeys; k4 += 4) {
+          float4 p[RT];
+#pragma unroll
+          for (int i = 0; i < RT; ++i) p[i] = *reinterpret_cast<const float4*>(P + (ty * RT + i) * kPStride + k4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+              const int c4 = tx + 16 * u;
+              if (c4 * 4 >= DP) continue;
+              const float4 v = *reinterpret_cast<const float4*>(V + tile_at(k4 + kk, c4, DP));
+#pragma unroll
+              for (int i = 0; i < RT; ++i) {
+                const float pk = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
+                if (decltype(masked)::value && pk < 0.0f) continue;
+                o[i][u][0] = fmaf(pk, v.x, o[i][u][0]);
+                o[i][u][1] = fmaf(pk, v.y, o[i][u][1]);
+                o[i][u][2] = fmaf(pk, v.z, o[i][u][2]);
+                o[i][u][3] = fmaf(pk, v.w, o[i][u][3]);
+              }
+            }
+        }
+      };
+      if (whole) accumulate(std::false_type{});
+      else accumulate(std::true_type{});
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty * RT + i;
+      if (r >= rows) continue;
+      const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+      const size_t at = (size_t)(q0 + t) * Hq + hq;
+      const bool none = l[i] == 0.0f;
+      const float inv = none ? 0.0f : 1.0f / l[i];
+      if (tx == 0) {
+        if (g.part >= 0) {
+          float* ml = a.part_ml + ((size_t)g.part * BR + r) * 2;
+          ml[0] = m[i];
+          ml[1] = l[i];
+        } else if (a.lse) {
+          a.lse[at] = none ? -INFINITY : (m[i] + log2f(l[i])) * (float)M_LN2;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 4 * (tx + 16 * u) + e;
+          if (c >= D) continue;
+          if (g.part >= 0) a.part_o[((size_t)g.part * BR + r) * D + c] = o[i][u][e];
+          else static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : o[i][u][e] * inv);
+        }
+    }
+  }
+}
+
+// Joins the segments of cut tiles: one warp per row, lanes over the columns.
+constexpr int kJoinWarps = 4;
+template <typename T, int NC>  // NC: columns per lane
+__global__ void __launch_bounds__(32 * kJoinWarps) k_paged_join(PagedAttn a, const PagedJoin* __restrict__ joins,
+                                                                int row_tile) {
+  const PagedJoin g = joins[blockIdx.x];
+  const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int q0 = __ldg(a.s.q_start + g.seq), nq = __ldg(a.s.q_start + g.seq + 1) - q0;
+  if (r >= min(row_tile, nq * a.group - g.row0)) return;
+  const int D = a.c.dim;
+  const float* ml = a.part_ml + ((size_t)g.part0 * row_tile + r) * 2;
+  float m = -INFINITY;
+  for (int p = lane; p < g.parts; p += 32) m = fmaxf(m, __ldg(ml + (size_t)p * row_tile * 2));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float mu = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, acc[NC];
+#pragma unroll
+  for (int u = 0; u < NC; ++u) acc[u] = 0.0f;
+  const float* po = a.part_o + ((size_t)g.part0 * row_tile + r) * D;
+#pragma unroll 4
+  for (int p = 0; p < g.parts; ++p) {
+    const float2 x = *reinterpret_cast<const float2*>(ml + (size_t)p * row_tile * 2);
+    const float w = exp2f(x.x - mu);
+    l = fmaf(w, x.y, l);
+#pragma unroll
+    for (int u = 0; u < NC; ++u) {
+      const int c = lane + 32 * u;
+      if (c < D) acc[u] = fmaf(w, __ldg(po + (size_t)p * row_tile * D + c), acc[u]);
+    }
+  }
+  const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+  const size_t at = (size_t)(q0 + t) * (a.c.heads * a.group) + hq;
+  const bool none = l == 0.0f;
+  if (lane == 0 && a.lse) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * (float)M_LN2;
+  const float inv = none ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int u = 0; u < NC; ++u) {
+    const int c = lane + 32 * u;
+    if (c < D) static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : acc[u] * inv);
+  }
+}
+
+// Attention weight of 64 slots of one (sequence, head): the column sums of
+// the softmax over all rows that may see them, each row's sum known from lse.
+// A CTA owns its slots and adds its rows in a fixed order: no atomics.
+template <typename T, int RT>
+__global__ void __launch_bounds__(kGenThreads) k_paged_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,
+                                                               float decay, int DP, bool wide, bool wide_q) {
+  constexpr int BR = 16 * RT;
+  extern __shared__ float4 sm4[];
+  float* K = reinterpret_cast<float*>(sm4);  // [64][DP]
+  float* Q = K + kGenKeys * DP;              // [BR][DP]
+  __shared__ float lse2[BR];
+  __shared__ float sums[16][kGenKeys];
+  const PagedSlots g = tiles[blockIdx.x];
+  const int h = blockIdx.y, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int D = a.c.dim, Hq = a.c.heads * a.group;
+  const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+  const int nq = __ldg(a.s.q_start + g.seq + 1) - q0;
+  const int* table = a.s.table + (size_t)g.seq * a.s.stride;
+  const int j0 = g.slot0, j1 = min(j0 + kGenKeys, n);
+  fill_tile<T>(K, kGenKeys, DP, D, wide, [&](int r) -> const T* {
+    return j0 + r < j1 ? static_cast<const T*>(a.c.keys) + paged_row(table, a.c, h, j0 + r) : nullptr;
+  });
+  // tokens that may see any of the slots: from slot j0 on, to the window's end
+  // behind the last slot unless some of the slots are sinks
+  const int ta = max(0, j0 - (n - nq));
+  const int tb = (a.window && j0 >= a.sinks) ? (int)min((long long)nq, (long long)j1 - 1 + a.window - (n - nq)) : nq;
+  float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int row0 = ta * a.group; row0 < tb * a.group; row0 += BR) {
+    const int rows = min(BR, tb * a.group - row0);
+    __syncthreads();
+    fill_tile<T>(Q, BR, DP, D, wide_q, [&](int r) -> const T* {
+      if (r >= rows) return nullptr;
+      const int t = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
+      return static_cast<const T*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
+    });
+    for (int r = tid; r < rows; r += kGenThreads) {
+      const int t = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
+      lse2[r] = a.lse[(size_t)(q0 + t) * Hq + hq] * (float)M_LOG2E;
+    }
+    __syncthreads();
+    float s[RT][4];
+    scores<RT>(Q, K, DP, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = ty * RT + i;
+      if (r >= rows) continue;
+      const float z = lse2[r];
+      if (z == -INFINITY) continue;  // a row that sees nothing
+      const int pos = n - nq + (row0 + r) / a.group;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (paged_sees(pos, j0 + tx + 16 * u, a.window, a.sinks)) w[u] += exp2f(fmaf(s[i][u], a.scale2, -z));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) sums[ty][tx + 16 * u] = w[u];
+  __syncthreads();
+  if (tid < j1 - j0) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sums[i][tid];
+    const int j = j0 + tid;
+    const int page = __ldg(table + (j >> a.c.page_shift));
+    float* p = a.c.weights + (((size_t)page * a.c.heads + h) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
+    *p = decay == 0.0f ? t : fmaf(decay, *p, t);
+  }
+}
+
+template <typename K>
+cudaError_t opt_in(K kern, size_t smem) {
+  if (smem <= kSmemOptIn) return cudaSuccess;
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+}
+
+// rows may be read 16 bytes at a time
+template <typename T>
+bool wide_rows(const PagedAttn& a) {
+  return a.c.dim * sizeof(T) % 16 == 0;
+}
+template <typename T>
+bool wide_query(const PagedAttn& a) {
+  return a.c.dim * sizeof(T) % 16 == 0 && (a.q_token | a.q_head) * sizeof(T) % 16 == 0 && aligned(a.q, 16);
+}
+
+template <typename T, int RT, int NU>
+cudaError_t attn_launch(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  const int DP = (a.c.dim + 31) / 32 * 32;
+  const size_t smem = ((size_t)(16 * RT + 2 * kGenKeys) * DP + 16 * RT * kPStride) * sizeof(float);
+  auto kern = k_paged_attn<T, RT, NU>;
+  cudaError_t e = opt_in(kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<w.ctas, kGenThreads, smem, st>>>(a, w.segs, w.first, DP, wide_rows<T>(a), wide_query<T>(a));
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t attn_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  const int nu = (a.c.dim + 63) / 64;
+  if (w.row_tile == kGenRows)
+    return nu == 1 ? attn_launch<T, 4, 1>(a, w, st) : nu == 2 ? attn_launch<T, 4, 2>(a, w, st)
+                                                              : attn_launch<T, 4, 4>(a, w, st);
+  return nu == 1 ? attn_launch<T, 1, 1>(a, w, st) : nu == 2 ? attn_launch<T, 1, 2>(a, w, st)
+                                                            : attn_launch<T, 1, 4>(a, w, st);
+}
+
+template <typename T>
+cudaError_t join_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  const dim3 grid((unsigned)w.joins_n, (unsigned)((w.row_tile + kJoinWarps - 1) / kJoinWarps));
+  if (a.c.dim <= 64) k_paged_join<T, 2><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
+  else if (a.c.dim <= 128) k_paged_join<T, 4><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
+  else k_paged_join<T, 8><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+template <typename T, int RT>
+cudaError_t weights_launch(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, float decay, cudaStream_t st) {
+  const int DP = (a.c.dim + 31) / 32 * 32;
+  const size_t smem = (size_t)(16 * RT + kGenKeys) * DP * sizeof(float);
+  auto kern = k_paged_weights<T, RT>;
+  cudaError_t e = opt_in(kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3((unsigned)ntiles, (unsigned)a.c.heads), kGenThreads, smem, st>>>(a, tiles, decay, DP, wide_rows<T>(a),
+                                                                              wide_query<T>(a));
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t weights_typed(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, bool few_rows, float decay,
+                          cudaStream_t st) {
+  return few_rows ? weights_launch<T, 1>(a, tiles, ntiles, decay, st)
+                  : weights_launch<T, 4>(a, tiles, ntiles, decay, st);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attn_generic(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  if (w.ctas == 0) return cudaSuccess;
+  if (a.c.dtype == KVF_IN_F32) return attn_typed<float>(a, w, st);
+  if (a.c.dtype == KVF_IN_F16) return attn_typed<__half>(a, w, st);
+  return attn_typed<__nv_bfloat16>(a, w, st);
+}
+
+cudaError_t launch_paged_join(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  if (w.joins_n == 0) return cudaSuccess;
+  if (a.c.dtype == KVF_IN_F32) return join_typed<float>(a, w, st);
+  if (a.c.dtype == KVF_IN_F16) return join_typed<__half>(a, w, st);
+  return join_typed<__nv_bfloat16>(a, w, st);
+}
+
+cudaError_t launch_paged_weights_generic(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, bool few_rows,
+                                         float decay, cudaStream_t st) {
+  if (ntiles == 0) return cudaSuccess;
+  if (a.c.dtype == KVF_IN_F32) return weights_typed<float>(a, tiles, ntiles, few_rows, decay, st);
+  if (a.c.dtype == KVF_IN_F16) return weights_typed<__half>(a, tiles, ntiles, few_rows, decay, st);
+  return weights_typed<__nv_bfloat16>(a, tiles, ntiles, few_rows, decay, st);
+}
+
+}  // namespace kvf
