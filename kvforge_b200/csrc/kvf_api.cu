@@ -25,6 +25,7 @@
 
 #include "kvf_internal.cuh"
 #include "kvf_paged.cuh"
+#include "kvf_paged_tc.cuh"
 
 using namespace kvf;
 
@@ -998,9 +999,14 @@ struct kvf_paged_plan {
   void* block = nullptr;  // device: tables and work lists
   PagedSeqs seqs;
   std::vector<PagedWork> works;
-  const PagedSlots* slots = nullptr;  // tiles of slots whose weights change
-  size_t slots_n = 0;
-  bool few_rows = false;  // every sequence has at most kGenRowsShort rows per KV head
+  // tiles of slots whose weights change: of sequences that the CUDA-core
+  // kernel sums, and of those whose scores k_paged_decode keeps
+  const PagedSlots* slots = nullptr;
+  const PagedSlots* decode_slots = nullptr;
+  size_t slots_n = 0, decode_slots_n = 0;
+  bool few_rows = false;  // every sequence among `slots` has at most kGenRowsShort rows per KV head
+  const long long* score_at = nullptr;  // [n] where a sequence's scores start
+  size_t scores_n = 0;
   cudaEvent_t ready = nullptr;
   mutable std::mutex use_mu;
   mutable std::vector<std::pair<cudaStream_t, cudaEvent_t>> uses;
@@ -1123,23 +1129,42 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   struct Offsets { size_t segs, first, joins; };
   std::vector<Offsets> at;
   std::vector<PagedWorkHost> hosts;
-  std::vector<PagedSlots> slots;
+  std::vector<PagedSlots> slots, decode_slots;
+  std::vector<long long> score_at;
   if (query_heads && tokens) {
     int sms = 0;
     KVF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device));
     const int group = (int)p->group, heads = (int)p->heads;
     hosts.resize(2);
-    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, kGenRowsShort, kGenRowsShort, kGenKeys,
-                3 * sms, 2, 1, &hosts[0]);
-    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, kGenRowsShort + 1, (long long)kMaxLen, kGenRows,
-                kGenKeys, 2 * sms, 2, 1, &hosts[1]);
+    const bool tc = paged_tc_fits(p->dtype, p->dim);
+    const long long few = kDecodeRows;
+    static_assert(kDecodeRows == kGenRowsShort, "the same sequences have few rows for both kernels");
+    if (tc) {
+      // two CTAs per SM
+      hosts[0].kernel = kPagedDecode;
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kDecodeRows, kDecodeKeys, 2 * sms, 2, 1,
+                  &hosts[0]);
+    } else {
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1,
+                  &hosts[0]);
+    }
+    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kGenRows, kGenKeys,
+                2 * sms, 2, 1, &hosts[1]);
     p->few_rows = hosts[1].segs.empty();
-    for (size_t i = 0; i < n; ++i)
-      if (q_lens[i])
-        for (int j = 0; j < kv_lens[i]; j += kGenKeys) slots.push_back({(int)i, j});
+    score_at.assign(n, 0);
+    for (size_t i = 0; i < n; ++i) {
+      if (!q_lens[i]) continue;
+      const bool decode = tc && (long long)q_lens[i] * group <= few;
+      const int step = decode ? kDecodeWeightSlots : kGenKeys;
+      for (int j = 0; j < kv_lens[i]; j += step) (decode ? decode_slots : slots).push_back({(int)i, j});
+      if (decode) {
+        score_at[i] = (long long)p->scores_n;
+        p->scores_n += (size_t)heads * q_lens[i] * group * kv_lens[i];
+      }
+    }
     for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});
   }
-  const size_t at_slots = img.add(slots);
+  const size_t at_slots = img.add(slots), at_decode_slots = img.add(decode_slots), at_score_at = img.add(score_at);
 
   KVF_CUDA(cudaMallocFromPoolAsync(&p->block, img.bytes.size(), p->ctx->pool, p->stream));
   KVF_TRY(upload(p->ctx, p->block, img.bytes.data(), img.bytes.size(), p->stream));
@@ -1153,6 +1178,7 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     const PagedWorkHost& h = hosts[i];
     if (h.segs.empty()) continue;
     PagedWork w;
+    w.kernel = h.kernel;
     w.row_tile = h.row_tile;
     w.key_tile = h.key_tile;
     w.ctas = (int)h.first.size() - 1;
@@ -1166,6 +1192,9 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   }
   p->slots = reinterpret_cast<const PagedSlots*>(d + at_slots);
   p->slots_n = slots.size();
+  p->decode_slots = reinterpret_cast<const PagedSlots*>(d + at_decode_slots);
+  p->decode_slots_n = decode_slots.size();
+  p->score_at = reinterpret_cast<const long long*>(d + at_score_at);
   KVF_CUDA(p->ctx->order_event(&p->ready));
   KVF_CUDA(cudaEventRecord(p->ready, p->stream));
   return KVF_OK;
@@ -2477,6 +2506,11 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
     a.lse = sc.get<float>(plan->tokens * plan->heads * plan->group);
     if (!a.lse) return fail(KVF_ERR_CUDA, "scratch allocation failed");
   }
+  float* scores = nullptr;
+  if (decay >= 0.0f && plan->decode_slots_n) {
+    scores = sc.get<float>(plan->scores_n);
+    if (!scores) return fail(KVF_ERR_CUDA, "scratch allocation failed");
+  }
   KVF_TRY(reader_enter(plan, st));
   cudaError_t err = cudaSuccess;
   for (const PagedWork& w : plan->works) {
@@ -2486,11 +2520,15 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
       a.part_ml = sc.get<float>(rows * 2);
       if (!a.part_o || !a.part_ml) err = cudaErrorMemoryAllocation;
     }
-    if (err == cudaSuccess) err = launch_paged_attn_generic(a, w, st);
+    if (err == cudaSuccess)
+      err = w.kernel == kPagedDecode ? launch_paged_decode(a, w, scores, plan->score_at, st)
+                                     : launch_paged_attn_generic(a, w, st);
     if (err == cudaSuccess) err = launch_paged_join(a, w, st);
   }
   if (err == cudaSuccess && decay >= 0.0f)
     err = launch_paged_weights_generic(a, plan->slots, plan->slots_n, plan->few_rows, decay, st);
+  if (err == cudaSuccess && decay >= 0.0f)
+    err = launch_paged_decode_weights(a, plan->decode_slots, plan->decode_slots_n, scores, plan->score_at, decay, st);
   const kvf_status ls = reader_leave(plan, st);
   KVF_CUDA(err);
   return ls;

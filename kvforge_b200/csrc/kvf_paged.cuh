@@ -44,7 +44,9 @@ struct PagedJoin {
 struct PagedSlots {
   int seq, slot0;
 };
+enum PagedKernel { kPagedGeneric = 0, kPagedDecode = 1, kPagedChunk = 2 };
 struct PagedWork {
+  int kernel = kPagedGeneric;
   int row_tile = 0, key_tile = 0;
   int ctas = 0, segs_n = 0, joins_n = 0, parts = 0;
   const PagedSeg* segs = nullptr;  // device
@@ -100,6 +102,7 @@ struct PagedAttn {
 
 // host side of a work list
 struct PagedWorkHost {
+  int kernel = kPagedGeneric;
   int row_tile = 0, key_tile = 0, parts = 0;
   std::vector<PagedSeg> segs;
   std::vector<int> first;
@@ -131,6 +134,19 @@ cudaError_t launch_paged_join(const PagedAttn& a, const PagedWork& w, cudaStream
 // logarithm): CUDA cores, every type; slots: tiles of kGenKeys slots
 cudaError_t launch_paged_weights_generic(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, bool few_rows,
                                          float decay, cudaStream_t st);
+
+// 16-bit pools with head dims of whole 16-byte rows up to 128, sequences of at
+// most kDecodeRows rows per KV head; scores (or nullptr): see the kernel
+constexpr int kDecodeRows = 16, kDecodeKeys = 64;
+constexpr int kDecodeWeightSlots = 256;  // slots of a tile of launch_paged_decode_weights
+cudaError_t launch_paged_decode(const PagedAttn& a, const PagedWork& w, float* scores, const long long* score_at,
+                                cudaStream_t st);
+cudaError_t launch_paged_decode_weights(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles,
+                                        const float* scores, const long long* score_at, float decay, cudaStream_t st);
+
+// the same pools, sequences of more rows
+constexpr int kChunkRows = 256, kChunkKeys = 128;
+cudaError_t launch_paged_chunk(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
 
 #ifdef __CUDACC__
 template <typename T>

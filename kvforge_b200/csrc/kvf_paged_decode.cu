@@ -1,0 +1,467 @@
+// Attention of few rows (single tokens, short drafts) over a paged 16-bit
+// cache: at most 16 query rows per KV head and sequence.
+//
+// The formulas are those of kvf_paged_attn.cu. Every key and value is read
+// once for up to 16 rows, so the kernel is bound by HBM; its products run on
+// mma.sync m16n8k16 with the rows as M (tcgen05's M of 128 would be mostly
+// padding, and the tensor cores are not what limits here). One producer warp
+// keeps tensor-map loads of 64-slot tiles in flight, a box per page; four
+// consumer warps take 16 slots each, with a running maximum and sum of their
+// own, and are joined once per segment. Two CTAs per SM keep about 190 KB of
+// loads in flight, four times what the latency-bandwidth product asks for.
+//
+// Slots that no row sees are masked by selection, and their values are
+// replaced by zeros in shared memory, whatever the pages hold. A non-finite
+// value that only some of the rows see is replaced as well and added, to the
+// rows that see it, at the end: its product with any positive weight is the
+// value itself.
+#include <algorithm>
+#include <cmath>
+
+#include "kvf_paged_tc.cuh"
+
+namespace kvf {
+namespace {
+
+constexpr int kRows = kDecodeRows, kKeys = kDecodeKeys;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * (kWarps + 1);
+template <int DP>
+constexpr int stages() { return DP == 128 ? 3 : 6; }
+template <int DP>
+constexpr int tile_bytes() { return kKeys * DP * 2; }
+template <int DP>
+constexpr size_t smem_bytes() {
+  return 1024 + (size_t)stages<DP>() * 2 * tile_bytes<DP>() + kRows * DP * sizeof(float);
+}
+
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// byte offset of 16-byte chunk `chunk` (8 columns) of slot `row` in a tile:
+// halves of 64 columns, 128 bytes a row, chunks permuted by the row
+__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// scores != nullptr: every score (base 2, -inf where unseen) is also written,
+// for the attention weights: sequence i's at scores + score_at[i], [head][row][slot]
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 2)
+    k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttn a,
+                   const PagedSeg* __restrict__ segs, const int* __restrict__ first, float* __restrict__ scores,
+                   const long long* __restrict__ score_at) {
+  constexpr int kStages = stages<DP>(), kTile = tile_bytes<DP>(), kSteps = DP / 16, kCols = DP / 8;
+  extern __shared__ uint8_t sm_raw[];
+  // the 128-byte swizzle takes its pattern from address bits 7-9
+  uint8_t* sm = sm_raw + ((1024u - (ptx::smem(sm_raw) & 1023u)) & 1023u);
+  float* merged = reinterpret_cast<float*>(sm + (size_t)kStages * 2 * kTile);  // [kRows][DP]
+  __shared__ uint64_t bars[2 * kStages];
+  __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
+  // whether a segment's tiles held non-finite values (by the segment's parity:
+  // the other one is cleared meanwhile), whether its consumers gave up
+  __shared__ int sh_bad[2], sh_stop;
+  __shared__ int sh_abort;
+  volatile int* abort_flag = &sh_abort;
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const uint32_t full = ptx::smem(bars), empty = ptx::smem(bars + kStages);
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      ptx::mbar_init(full + 8 * i, 1);
+      ptx::mbar_init(empty + 8 * i, kWarps);
+    }
+    sh_abort = sh_stop = sh_bad[0] = sh_bad[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  const int seg0 = __ldg(first + blockIdx.x), seg1 = __ldg(first + blockIdx.x + 1);
+  const int box = min(kKeys, 1 << a.c.page_shift);  // slots of one load
+  bool gave_up = false;
+
+  if (w == kWarps) {
+    // ---------------- producer: one lane per box of a tile ----------------
+    int n_tile = 0, pending = 0;
+    for (int si = seg0; si < seg1 && !gave_up; ++si) {
+      const PagedSeg g = segs[si];
+      const int n = __ldg(a.s.kv_len + g.seq);
+      const int nq = __ldg(a.s.q_start + g.seq + 1) - __ldg(a.s.q_start + g.seq);
+      const int* table = a.s.table + (size_t)g.seq * a.s.stride;
+      const PagedSpan span = paged_span(g.row0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
+      for (int it = g.it0; it < g.it1; ++it, ++n_tile) {
+        const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys;
+        const int j = j0 + lane * box;
+        const bool mine = lane * box < kKeys && j < n;
+        const int page = mine ? __ldg(table + (j >> a.c.page_shift)) : 0;
+        const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+        const int s = n_tile % kStages, round = n_tile / kStages;
+        if (round > 0 && !mbar_wait_bounded(empty + 8 * s, (round - 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (__any_sync(0xffffffffu, gave_up)) {
+          gave_up = true;
+          break;
+        }
+        if (lane == 0) ptx::mbar_expect(full + 8 * s, (uint32_t)(boxes * 2 * box * DP * 2));
+        __syncwarp();
+        if (mine) {
+          const uint32_t dst = ptx::smem(sm) + (uint32_t)(s * 2 * kTile + lane * box * 128);
+          const int y = j & ((1 << a.c.page_shift) - 1), z = page * a.c.heads + g.head;
+#pragma unroll
+          for (int half = 0; half < DP / 64; ++half) {
+            ptx::load_box(dst + half * (kKeys * 128), &kmap, 64 * half, y, z, full + 8 * s);
+            ptx::load_box(dst + kTile + half * (kKeys * 128), &vmap, 64 * half, y, z, full + 8 * s);
+          }
+        }
+        pending = n_tile + 1;
+      }
+    }
+    // after a timeout the loads in flight still land in this CTA's memory
+    if (gave_up) {
+      *abort_flag = 1;
+      for (int t = max(0, pending - kStages); t < pending; ++t)
+        mbar_wait_bounded(full + 8 * (t % kStages), (t / kStages) & 1, kWaitNs);
+    }
+  } else {
+    // ---------------- consumers ----------------
+    const int r0 = lane >> 2, c0 = (lane & 3) * 2;  // rows r0, r0 + 8; columns c0, c0 + 1 of an 8-wide tile
+    const int Hq = a.c.heads * a.group, D = a.c.dim;
+    int n_tile = 0;
+    for (int si = seg0; si < seg1; ++si) {
+      const PagedSeg g = segs[si];
+      const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+      const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = min(kRows, nq * a.group - g.row0);
+      const PagedSpan span = paged_span(g.row0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
+      uint32_t qf[kSteps][4];
+      int pos[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 8 * i;
+        const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+        pos[i] = n - nq + t;
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
+        const bool pair = (reinterpret_cast<uintptr_t>(p) & 3) == 0;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = 16 * k + 8 * e + c0;
+            uint32_t x = 0;
+            if (r < rows && c < D) {  // D is even
+              if (pair) x = __ldg(reinterpret_cast<const uint32_t*>(p + c));
+              else x = (uint32_t)__ldg(p + c) | ((uint32_t)__ldg(p + c + 1) << 16);
+            }
+            qf[k][2 * e + i] = x;
+          }
+      }
+      const int pa = n - nq + g.row0 / a.group, pb = n - nq + (g.row0 + rows - 1) / a.group;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kCols][4];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
+      float* sc = scores ? scores + score_at[g.seq] + ((size_t)g.head * nq * a.group + g.row0) * n : nullptr;
+
+      for (int it = g.it0; it < g.it1; ++it, ++n_tile) {
+        const int s = n_tile % kStages;
+        const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys + 16 * w;  // this warp's slots
+        const uint32_t kt = ptx::smem(sm) + (uint32_t)(s * 2 * kTile), vt = kt + kTile;
+        if (!mbar_wait_bounded(full + 8 * s, (n_tile / kStages) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (__any_sync(0xffffffffu, gave_up)) {
+          gave_up = true;
+          break;
+        }
+        float x[2][4] = {};
+        {
+          const int row = 16 * w + ((lane >> 4) << 3) + (lane & 7), odd = (lane >> 3) & 1;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            uint32_t b[4];
+            ldsm4(kt + tile_off(row, 2 * k + odd), b);
+            mma16816<T>(x[0], qf[k], b[0], b[1]);
+            mma16816<T>(x[1], qf[k], b[2], b[3]);
+          }
+        }
+        // slots that every row sees need no masks
+        const bool whole = j0 + 15 <= pa && (!a.window || j0 > pb - a.window || j0 + 16 <= a.sinks);
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[t][e] *= a.scale2;
+            if (!whole && !paged_sees(pos[e >> 1], j0 + 8 * t + c0 + (e & 1), a.window, a.sinks)) x[t][e] = -INFINITY;
+            mx[e >> 1] = fmaxf(mx[e >> 1], x[t][e]);
+          }
+        if (sc) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = r0 + 8 * (e >> 1), j = j0 + 8 * t + c0 + (e & 1);
+              if (r < rows && j < n) sc[(size_t)r * n + j] = x[t][e];
+            }
+        }
+        float f[2], mu[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+          mu[i] = mx[i] == -INFINITY ? 0.0f : mx[i];
+          f[i] = ex2(m[i] - mu[i]);
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            l[i] *= f[i];
+            m[i] = mx[i];
+          }
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            o[c][0] *= f[0];
+            o[c][1] *= f[0];
+            o[c][2] *= f[1];
+            o[c][3] *= f[1];
+          }
+        }
+        float p[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[t][e] = ex2(x[t][e] - mu[e >> 1]);
+            l[e >> 1] += p[t][e];
+          }
+        // the numerators are rounded to the cache's type for the product with
+        // the values; the sum keeps them in f32
+        const uint32_t pf[4] = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]),
+                                pack2<T>(p[1][2], p[1][3])};
+        if (!whole) {  // this warp's 16 rows of V, two lanes a row
+          const int row = lane >> 1, j = j0 + row;
+          const bool any = j <= pb && (!a.window || j > pa - a.window || j < a.sinks);
+          bool bad = false;
+#pragma unroll 1
+          for (int c = lane & 1; c < kCols; c += 2) {
+            uint4* q = reinterpret_cast<uint4*>(sm + (size_t)s * 2 * kTile + kTile + tile_off(16 * w + row, c));
+            if (!any) *q = make_uint4(0, 0, 0, 0);
+            else {
+              uint4 v = *q;
+              if (drop_nonfinite<T>(v)) {
+                *q = v;
+                bad = true;
+              }
+            }
+          }
+          if (bad) sh_bad[si & 1] = 1;
+          __syncwarp();
+        }
+        {
+          const int row = 16 * w + (lane & 15), odd = lane >> 4;
+#pragma unroll
+          for (int c = 0; c < kCols; c += 2) {
+            uint32_t b[4];
+            ldsm4t(vt + tile_off(row, c + odd), b);
+            mma16816<T>(o[c], pf, b[0], b[1]);
+            mma16816<T>(o[c + 1], pf, b[2], b[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
+      }
+      if (gave_up) {  // the other warps' waits end by it too
+        *abort_flag = 1;
+        sh_stop = 1;
+      }
+      // join the four warps: row maxima first, then the rescaled sums in order
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if ((lane & 3) == 0) {
+          sh_m[w][r0 + 8 * i] = m[i];
+          sh_l[w][r0 + 8 * i] = l[i];
+        }
+      }
+      consumer_sync();
+      if (tid == 0) sh_bad[(si + 1) & 1] = 0;
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float M = sh_m[0][r0 + 8 * i];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sh_m[k][r0 + 8 * i]);
+        f[i] = M == -INFINITY ? 0.0f : ex2(m[i] - M);
+      }
+      for (int k = 0; k < kWarps; ++k) {
+        if (w == k) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float2* q = reinterpret_cast<float2*>(merged + (r0 + 8 * i) * DP + 8 * c + c0);
+              float2 v = k ? *q : make_float2(0.0f, 0.0f);
+              v.x += o[c][2 * i] * f[i];
+              v.y += o[c][2 * i + 1] * f[i];
+              *q = v;
+            }
+        }
+        consumer_sync();
+      }
+      // read between two barriers, so that all warps go on or stop together
+      const bool bad = sh_bad[si & 1] != 0, stop = sh_stop != 0;
+      for (int i = tid; i < rows * DP; i += 32 * kWarps) {
+        const int r = i / DP, c = i - r * DP;
+        if (c >= D) continue;
+        float M = sh_m[0][r], L = 0.0f, v = merged[i];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sh_m[k][r]);
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) L += M == -INFINITY ? 0.0f : sh_l[k][r] * ex2(sh_m[k][r] - M);
+        const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+        if (bad) {  // non-finite values that were taken out of tiles that not every row sees whole
+          const int* table = a.s.table + (size_t)g.seq * a.s.stride;
+          for (int it = g.it0; it < g.it1; ++it) {
+            const int t0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys;
+            for (int j = t0; j < t0 + kKeys && j <= n - nq + t; ++j) {
+              const int b0 = j & ~15;
+              if ((b0 + 15 <= pa && (!a.window || b0 > pb - a.window || b0 + 16 <= a.sinks)) ||
+                  !paged_sees(n - nq + t, j, a.window, a.sinks))
+                continue;
+              const float y = to_float<T>(static_cast<const T*>(a.c.values)[paged_row(table, a.c, g.head, j) + c]);
+              if (!isfinite(y)) v += y;
+            }
+          }
+        }
+        const size_t at = (size_t)(q0 + t) * Hq + hq;
+        if (g.part >= 0) {
+          a.part_o[((size_t)g.part * kRows + r) * D + c] = v;
+          if (c == 0) {
+            a.part_ml[((size_t)g.part * kRows + r) * 2] = M;
+            a.part_ml[((size_t)g.part * kRows + r) * 2 + 1] = L;
+          }
+        } else {
+          const bool none = L == 0.0f;
+          static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : v / L);
+          if (c == 0 && a.lse) a.lse[at] = none ? -INFINITY : (M + log2f(L)) * (float)M_LN2;
+        }
+      }
+      consumer_sync();  // the joined sums are read before the next segment writes them
+      if (stop) break;
+    }
+  }
+  if (gave_up && a.status) atomicOr(a.status, kDevErrTimeout);
+}
+
+// Attention weights from the scores that k_paged_decode wrote: a thread per
+// slot adds its rows in order.
+constexpr int kWeightThreads = kDecodeWeightSlots;
+__global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,
+                                                                         const float* __restrict__ scores,
+                                                                         const long long* __restrict__ score_at,
+                                                                         float decay) {
+  __shared__ float lse2[kRows];
+  const PagedSlots g = tiles[blockIdx.x];
+  const int h = blockIdx.y, n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+  const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = nq * a.group;
+  if ((int)threadIdx.x < rows) {
+    const int t = threadIdx.x / a.group, hq = h * a.group + threadIdx.x % a.group;
+    lse2[threadIdx.x] = a.lse[(size_t)(q0 + t) * (a.c.heads * a.group) + hq] * (float)M_LOG2E;
+  }
+  __syncthreads();
+  const int j = g.slot0 + threadIdx.x;
+  if (j >= n) return;
+  // tiles that no row visits were not written
+  const PagedSpan span = paged_span(0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
+  const int tile = j / kKeys;
+  const bool there = tile < span.nsink || (tile >= span.first && tile < span.first + span.count - span.nsink);
+  float t = 0.0f;
+  if (there) {
+    const float* sc = scores + score_at[g.seq] + (size_t)h * rows * n + j;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const float z = lse2[r];
+      const float p = exp2f(__ldg(sc + (size_t)r * n) - z);
+      t += z == -INFINITY ? 0.0f : p;
+    }
+  }
+  const int page = __ldg(a.s.table + (size_t)g.seq * a.s.stride + (j >> a.c.page_shift));
+  float* p = a.c.weights + (((size_t)page * a.c.heads + h) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
+  *p = decay == 0.0f ? t : fmaf(decay, *p, t);
+}
+
+template <typename T, int DP>
+cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& vm, const PagedAttn& a, const PagedWork& w,
+                         float* scores, const long long* score_at, cudaStream_t st) {
+  auto kern = k_paged_decode<T, DP>;
+  constexpr size_t smem = smem_bytes<DP>();
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  kern<<<w.ctas, kThreads, smem, st>>>(km, vm, a, w.segs, w.first, scores, score_at);
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_decode(const PagedAttn& a, const PagedWork& w, float* scores, const long long* score_at,
+                                cudaStream_t st) {
+  if (w.ctas == 0) return cudaSuccess;
+  CUtensorMap km, vm;
+  const int rows = std::min(kKeys, 1 << a.c.page_shift);
+  if (!paged_map(&km, a.c, a.c.keys, rows) || !paged_map(&vm, a.c, a.c.values, rows)) return cudaErrorInvalidValue;
+  if (a.c.dtype == KVF_IN_F16)
+    return a.c.dim <= 64 ? launch_typed<__half, 64>(km, vm, a, w, scores, score_at, st)
+                         : launch_typed<__half, 128>(km, vm, a, w, scores, score_at, st);
+  return a.c.dim <= 64 ? launch_typed<__nv_bfloat16, 64>(km, vm, a, w, scores, score_at, st)
+                       : launch_typed<__nv_bfloat16, 128>(km, vm, a, w, scores, score_at, st);
+}
+
+cudaError_t launch_paged_decode_weights(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles,
+                                        const float* scores, const long long* score_at, float decay, cudaStream_t st) {
+  if (ntiles == 0) return cudaSuccess;
+  k_paged_decode_weights<<<dim3((unsigned)ntiles, (unsigned)a.c.heads), kWeightThreads, 0, st>>>(a, tiles, scores,
+                                                                                                score_at, decay);
+  note_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace kvf
