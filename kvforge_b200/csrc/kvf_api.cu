@@ -1148,8 +1148,15 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
       paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1,
                   &hosts[0]);
     }
-    paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kGenRows, kGenKeys,
-                2 * sms, 2, 1, &hosts[1]);
+    if (tc) {
+      // one CTA per SM; a segment's start and end cost about two tiles
+      hosts[1].kernel = kPagedChunk;
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kChunkRows,
+                  kChunkKeys, sms, 4, 2, &hosts[1]);
+    } else {
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kGenRows, kGenKeys,
+                  2 * sms, 2, 1, &hosts[1]);
+    }
     p->few_rows = hosts[1].segs.empty();
     score_at.assign(n, 0);
     for (size_t i = 0; i < n; ++i) {
@@ -2521,8 +2528,9 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
       if (!a.part_o || !a.part_ml) err = cudaErrorMemoryAllocation;
     }
     if (err == cudaSuccess)
-      err = w.kernel == kPagedDecode ? launch_paged_decode(a, w, scores, plan->score_at, st)
-                                     : launch_paged_attn_generic(a, w, st);
+      err = w.kernel == kPagedDecode  ? launch_paged_decode(a, w, scores, plan->score_at, st)
+            : w.kernel == kPagedChunk ? launch_paged_chunk(a, w, st)
+                                      : launch_paged_attn_generic(a, w, st);
     if (err == cudaSuccess) err = launch_paged_join(a, w, st);
   }
   if (err == cudaSuccess && decay >= 0.0f)
