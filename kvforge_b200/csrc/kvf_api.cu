@@ -1005,6 +1005,7 @@ struct kvf_paged_plan {
   const PagedSlots* decode_slots = nullptr;
   size_t slots_n = 0, decode_slots_n = 0;
   bool few_rows = false;  // every sequence among `slots` has at most kGenRowsShort rows per KV head
+  PagedWork weights;  // the same sequences as `slots`, for the tensor-core sums (joins_n 0: none)
   const long long* score_at = nullptr;  // [n] where a sequence's scores start
   size_t scores_n = 0;
   cudaEvent_t ready = nullptr;
@@ -1158,6 +1159,10 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
                   2 * sms, 2, 1, &hosts[1]);
     }
     p->few_rows = hosts[1].segs.empty();
+    if (tc && group <= 128) {
+      hosts.resize(3);
+      paged_split_slots(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few, sms, &hosts[2]);
+    }
     score_at.assign(n, 0);
     for (size_t i = 0; i < n; ++i) {
       if (!q_lens[i]) continue;
@@ -1183,7 +1188,7 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   p->seqs.n = (int)n;
   for (size_t i = 0; i < hosts.size(); ++i) {
     const PagedWorkHost& h = hosts[i];
-    if (h.segs.empty()) continue;
+    if (h.segs.empty() && h.joins.empty()) continue;
     PagedWork w;
     w.kernel = h.kernel;
     w.row_tile = h.row_tile;
@@ -1195,7 +1200,8 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     w.segs = reinterpret_cast<const PagedSeg*>(d + at[i].segs);
     w.first = reinterpret_cast<const int*>(d + at[i].first);
     w.joins = reinterpret_cast<const PagedJoin*>(d + at[i].joins);
-    p->works.push_back(w);
+    if (i == 2) p->weights = w;
+    else p->works.push_back(w);
   }
   p->slots = reinterpret_cast<const PagedSlots*>(d + at_slots);
   p->slots_n = slots.size();
@@ -2533,8 +2539,16 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
                                       : launch_paged_attn_generic(a, w, st);
     if (err == cudaSuccess) err = launch_paged_join(a, w, st);
   }
-  if (err == cudaSuccess && decay >= 0.0f)
-    err = launch_paged_weights_generic(a, plan->slots, plan->slots_n, plan->few_rows, decay, st);
+  if (err == cudaSuccess && decay >= 0.0f && plan->slots_n) {
+    err = cudaErrorNotSupported;
+    if (plan->weights.joins_n) {
+      float* part_w = sc.get<float>((size_t)plan->weights.parts * kWeightSlots);
+      err = part_w ? launch_paged_chunk_weights(a, plan->weights, plan->tokens, part_w, decay, st)
+                   : cudaErrorMemoryAllocation;
+    }
+    if (err == cudaErrorNotSupported)
+      err = launch_paged_weights_generic(a, plan->slots, plan->slots_n, plan->few_rows, decay, st);
+  }
   if (err == cudaSuccess && decay >= 0.0f)
     err = launch_paged_decode_weights(a, plan->decode_slots, plan->decode_slots_n, scores, plan->score_at, decay, st);
   const kvf_status ls = reader_leave(plan, st);

@@ -148,6 +148,16 @@ cudaError_t launch_paged_decode_weights(const PagedAttn& a, const PagedSlots* ti
 constexpr int kChunkRows = 256, kChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
 
+// their attention weights, from a.lse: up to 128 query heads per KV head;
+// part_w: w.parts * kWeightSlots floats. cudaErrorNotSupported (before any
+// launch) where the queries' strides or alignment do not suit tensor maps.
+// The work: tiles of kWeightSlots slots by row tiles of 128 / group tokens.
+constexpr int kWeightSlots = 256;
+void paged_split_slots(const int* q_lens, const int* kv_lens, size_t n, int heads, int group, int window, int sinks,
+                       long long more_than, int slots, PagedWorkHost* out);
+cudaError_t launch_paged_chunk_weights(const PagedAttn& a, const PagedWork& w, size_t tokens, float* part_w,
+                                       float decay, cudaStream_t st);
+
 #ifdef __CUDACC__
 template <typename T>
 __device__ __forceinline__ float to_float(T x);

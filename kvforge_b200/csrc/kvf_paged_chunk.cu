@@ -35,15 +35,14 @@
 namespace kvf {
 namespace {
 
+using namespace ptx;
+
 constexpr int kRows = kChunkRows, kKeys = kChunkKeys;
-constexpr int kTile = 128;  // rows of one row tile: MMA M, TMEM lanes
 constexpr int kTiles = kRows / kTile;
 constexpr int kThreads = 384;
-constexpr int kHalf = kTile * 128;  // bytes of 128 rows by 64 columns
 // registers per thread: launched with 168 (65536 / 384), the softmax warps take
 // what the others give up: 2 x 128 x 200 + 128 x 104 = 384 x 168
 constexpr int kRegsSoftmax = 200, kRegsOther = 104;
-constexpr uint32_t kTmemCols = 512;
 
 template <int DP>
 constexpr int tile_bytes() { return kTile * DP * 2; }
@@ -53,96 +52,6 @@ template <int DP>
 constexpr size_t smem_bytes() { return 1024 + (size_t)(kTiles + stages<DP>()) * tile_bytes<DP>(); }
 // more than half of an SM's shared memory: one CTA per SM, whose TMEM is free
 static_assert(2 * (smem_bytes<64>() + 1024) > 228 * 1024 && smem_bytes<128>() + 2048 <= 227 * 1024 + 1024, "one CTA");
-
-// shared-memory matrix descriptors, 128-byte swizzle: 8-slot groups 1024 bytes
-// apart. K-major (Q, K): 64 columns per 128-byte row. MN-major (V as the
-// second product's B, whose N runs along the row): 64-column halves kHalf apart.
-constexpr uint64_t kDescBase = ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | kDescBase;
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kHalf >> 4) << 16) | kDescBase;
-}
-// instruction descriptor: f32 accumulators, A and B of type T, M = 128
-template <typename T>
-constexpr uint32_t idesc(int n, bool b_mn) {
-  const uint32_t t = std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(kTile >> 4) << 24);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 32 columns of this thread's TMEM lane
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-      "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
-        "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
-        "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
-  const uint32_t* u = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
-      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
-      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};" ::"r"(taddr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-// byte offset of 16-byte chunk `chunk` (8 columns) of row `row` of a tile
-__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
-  return (uint32_t)((chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-}
 
 // a segment as its roles see it
 struct Seg {
@@ -174,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const PagedSeg* __restrict__ segs, const int* __restrict__ first, bool wide_q, bool wide_out) {
   constexpr int kStages = stages<DP>(), kBytes = tile_bytes<DP>();
   extern __shared__ uint8_t sm_raw[];
-  uint8_t* sm = sm_raw + ((1024u - (ptx::smem(sm_raw) & 1023u)) & 1023u);
+  uint8_t* sm = sm_raw + ((1024u - (smem(sm_raw) & 1023u)) & 1023u);
   uint8_t* ring = sm + kTiles * kBytes;
   __shared__ uint64_t bars[3 * kStages + 4 * kTiles + 1];
   __shared__ uint32_t sh_tmem;
@@ -183,29 +92,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   // segment's index mod 8 (loads run less than three segments ahead)
   __shared__ int sh_bad[8];
   volatile int* abort_flag = &sh_abort;
-  const uint32_t full = ptx::smem(bars), empty = full + 8 * kStages, fixed = empty + 8 * kStages;
+  const uint32_t full = smem(bars), empty = full + 8 * kStages, fixed = empty + 8 * kStages;
   const uint32_t q_full = fixed + 8 * kStages, s_full = q_full + 8 * kTiles, p_ready = s_full + 8 * kTiles,
                  o_full = p_ready + 8 * kTiles, drained = o_full + 8 * kTiles;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
 
   if (w == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ptx::smem(&sh_tmem)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem(&sh_tmem)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      ptx::mbar_init(full + 8 * i, 1);
-      ptx::mbar_init(empty + 8 * i, 3);  // the MMAs' completion and warps 10 and 11
-      ptx::mbar_init(fixed + 8 * i, 2);
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 3);  // the MMAs' completion and warps 10 and 11
+      mbar_init(fixed + 8 * i, 2);
     }
     for (int i = 0; i < kTiles; ++i) {
-      ptx::mbar_init(q_full + 8 * i, kTile);
-      ptx::mbar_init(s_full + 8 * i, 1);
-      ptx::mbar_init(p_ready + 8 * i, 4);
-      ptx::mbar_init(o_full + 8 * i, 1);
+      mbar_init(q_full + 8 * i, kTile);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_ready + 8 * i, 4);
+      mbar_init(o_full + 8 * i, 1);
     }
-    ptx::mbar_init(drained, 1);
+    mbar_init(drained, 1);
     sh_abort = 0;
     for (int i = 0; i < 8; ++i) sh_bad[i] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -234,13 +143,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           gave_up = true;
           return;
         }
-        if (lane == 0) ptx::mbar_expect(full + 8 * st, (uint32_t)(boxes * box * DP * 2));
+        if (lane == 0) mbar_expect(full + 8 * st, (uint32_t)(boxes * box * DP * 2));
         __syncwarp();
         if (mine) {
-          const uint32_t dst = ptx::smem(ring) + (uint32_t)(st * kBytes + lane * box * 128);
+          const uint32_t dst = smem(ring) + (uint32_t)(st * kBytes + lane * box * 128);
 #pragma unroll
           for (int half = 0; half < DP / 64; ++half)
-            ptx::load_box(dst + half * kHalf, map, 64 * half, j & (page - 1), p * a.c.heads + s.g.head, full + 8 * st);
+            load_box(dst + half * kHalf, map, 64 * half, j & (page - 1), p * a.c.heads + s.g.head, full + 8 * st);
         }
         ++n_tile;
       };
@@ -270,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return !gave_up;
         };
         auto scores = [&](int i, int st) {
-          const uint32_t q = ptx::smem(sm) + i * kBytes, k = ptx::smem(ring) + st * kBytes;
+          const uint32_t q = smem(sm) + i * kBytes, k = smem(ring) + st * kBytes;
 #pragma unroll
           for (int ks = 0; ks < DP / 16; ++ks) {
             const uint32_t off = (ks >> 2) * kHalf + (ks & 3) * 32;
@@ -305,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < nt; ++i) {
               if (!wait(p_ready + 8 * i, cnt_p[i]++)) break;
               fence_after();
-              const uint32_t v = ptx::smem(ring) + sv * kBytes;
+              const uint32_t v = smem(ring) + sv * kBytes;
 #pragma unroll
               for (int ks = 0; ks < kKeys / 16; ++ks)
                 mma_ts(tmem + 256 + i * DP, tmem + i * 128 + ks * 8, desc_mn(v + ks * 2048), idesc<T>(DP, true),
@@ -367,9 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (bad) sh_bad[si & 7] = si;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what was written
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(fixed + 8 * st);
+            if (lane == 0) mbar_arrive(fixed + 8 * st);
           }
-          if (lane == 0) ptx::mbar_arrive(empty + 8 * st);
+          if (lane == 0) mbar_arrive(empty + 8 * st);
         }
       }
       if (gave_up) *abort_flag = 1;
@@ -417,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(sm + i * kBytes + tile_off(t, ch)) = x;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        ptx::mbar_arrive(q_full + 8 * i);
+        mbar_arrive(q_full + 8 * i);
       }
       // the slots of this row tile's first and last query
       const int pa = s.n - s.nq + (s.g.row0 + i * kTile) / a.group;
@@ -490,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_ready + 8 * i);
+        if (lane == 0) mbar_arrive(p_ready + 8 * i);
       }
       if (gave_up) break;
       if (count > 0) {
@@ -579,11 +488,11 @@ template <typename T, int DP>
 cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& vm, const PagedAttn& a, const PagedWork& w,
                          cudaStream_t st) {
   auto kern = k_paged_chunk<T, DP>;
-  constexpr size_t smem = smem_bytes<DP>();
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr size_t bytes = smem_bytes<DP>();
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
   const bool wide_q = (a.q_token | a.q_head) % 8 == 0 && aligned(a.q, 16);
-  kern<<<w.ctas, kThreads, smem, st>>>(km, vm, a, w.segs, w.first, wide_q, aligned(a.out, 16));
+  kern<<<w.ctas, kThreads, bytes, st>>>(km, vm, a, w.segs, w.first, wide_q, aligned(a.out, 16));
   note_launches(1);
   return cudaGetLastError();
 }

@@ -377,6 +377,26 @@ def test_strides(kvf, dtype):
         check(w, q2)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D,heads,group,lens", [(128, 2, 5, [(300, 100), (3, 1)]), (64, 1, 3, [(1000, 600)]),
+                                                (128, 1, 150, [(200, 30), (64, 1)])])
+def test_weights_of_strided_queries(kvf, dtype, D, heads, group, lens):
+    """Rows that start at odd elements, or lie apart by odd strides, and more
+    query heads per KV head than a tile has rows."""
+    w = World(kvf, lens, heads, D, dtype, 32, seed=13)
+    q = w.step(heads * group)
+    n = q.shape[0]
+    box = torch.empty(n * heads * group * (D + 1) + 1, device="cuda", dtype=dtype)
+    q2 = box[1:].view(n, heads * group, D + 1)[:, :, :D]
+    q2.copy_(q)
+    check(w, q2, decay=0.0)
+    wide = torch.zeros((n, heads * group, 2 * D), device="cuda", dtype=dtype)
+    wide[:, :, D:] = q
+    check(w, wide[:, :, D:], decay=0.0)
+    one = q[:, :1].expand(n, heads * group, D)
+    check(w, one, decay=0.0)
+
+
 def test_other_streams(kvf):
     """Tokens appended on one stream are there for a call on another."""
     lens, H, G, D, page = SHAPES[14]
