@@ -65,7 +65,7 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
     if ((int)out->segs.size() > out->first.back()) out->first.push_back((int)out->segs.size());
     // a quota of a whole number of tiles may need a few CTAs more; they only
     // cost a wave when the extra ones do not fit beside the others
-    if ((int)out->first.size() - 1 <= slots || attempt == 8) return;
+    if ((int)out->first.size() - 1 <= slots || attempt == 16) return;
     quota += std::max<long long>(1, quota / 32);
   }
 }

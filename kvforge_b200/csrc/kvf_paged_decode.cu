@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int page = mine ? __ldg(table + (j >> a.c.page_shift)) : 0;
         const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
         const int s = n_tile % kStages, round = n_tile / kStages;
-        if (round > 0 && !mbar_wait_bounded(empty + 8 * s, (round - 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (round > 0 && !ptx::mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
           break;
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int s = n_tile % kStages;
         const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys + 16 * w;  // this warp's slots
         const uint32_t kt = ptx::smem(sm) + (uint32_t)(s * 2 * kTile), vt = kt + kTile;
-        if (!mbar_wait_bounded(full + 8 * s, (n_tile / kStages) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (!ptx::mbar_wait(full + 8 * s, (n_tile / kStages) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
           break;

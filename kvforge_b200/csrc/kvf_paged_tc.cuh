@@ -44,6 +44,21 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// mbar_wait_bounded behind a first few polls that read neither the clock nor the
+// flag: a poll takes about 110 cycles here even when the phase is complete, and
+// the rest of the loop should add little to it
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 128;\n"
+      "WAIT:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+      " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra WAIT;\n"
+      "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done || mbar_wait_bounded(bar, parity, kWaitNs, abort_flag);
+}
 // one box: columns x.., slots y.. of (page, head) z
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -60,16 +75,13 @@ constexpr uint32_t kTmemCols = 512;
 __device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
   return (uint32_t)((chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
-// shared-memory matrix descriptors, 128-byte swizzle: 8-slot groups 1024 bytes
-// apart. K-major (Q, K): 64 columns per 128-byte row. MN-major (V as the
-// second product's B, whose N runs along the row): 64-column halves kHalf apart.
-constexpr uint64_t kDescBase = ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | kDescBase;
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(kHalf >> 4) << 16) | kDescBase;
-}
+// Shared-memory matrix descriptors, 128-byte swizzle: 8-row groups 1024 bytes
+// apart. K-major (Q, K): 64 columns per 128-byte row. MN-major (V as the second
+// product's B, whose N runs along the row): 64-column halves kHalf apart. Only
+// the low word depends on the address; steps along an operand are added to it.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | ((uint32_t)(kHalf >> 4) << 16); }
 // instruction descriptor: f32 accumulators, A and B of type T, M = 128
 template <typename T>
 constexpr uint32_t idesc(int n, bool b_mn) {
@@ -77,22 +89,34 @@ constexpr uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kTile >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// The MMA warp runs its loop with all lanes, so that addresses and descriptors
+// stay in uniform registers (one lane alone in a branch took several hundred
+// cycles per tile to move them there); `lead` holds on the one lane that issues.
+__device__ __forceinline__ void mma_ss(bool lead, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n .reg .pred p, e;\n .reg .b64 da, db;\n setp.ne.b32 e, %0, 0;\n setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 da, {%2, %6};\n mov.b64 db, {%3, %6};\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %4, p;\n}\n" ::"r"((uint32_t)lead),
+      "r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(bool lead, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
+      "{\n .reg .pred p, e;\n .reg .b64 db;\n setp.ne.b32 e, %0, 0;\n setp.ne.b32 p, %5, 0;\n"
+      " mov.b64 db, {%3, %6};\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], db, %4, p;\n}\n" ::"r"((uint32_t)lead),
+      "r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void commit(bool lead, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %0, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}\n" ::"r"((uint32_t)lead),
+      "r"(bar)
+      : "memory");
 }
+// the same value on every lane, known as such to the compiler
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -130,10 +154,46 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// the largest of three (one instruction on sm_100), NaN if any is
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+  return d;
+}
+// two additions in one instruction, each rounded as usual
+__device__ __forceinline__ float2 fadd2(float2 x, float2 y) {
+  unsigned long long a, b, d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(y.x), "f"(y.y));
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^y of two values on the multiply-add units instead of the exponential unit
+// (16 per cycle and SM): 2^n * 2^f with n = round(y) and f = y - n in [-1/2, 1/2],
+// 2^f = 1 + f q(f) with q of degree 4 fitted for the least relative error by
+// linear programming on 4001 points; off by at most 1.7e-7 in all, as ex2.approx.
+// 0 below 2^-127; NaN is NOT handed on (the callers see to it).
+__device__ __forceinline__ float2 ex2_fma(float2 y) {
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.x));  // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.y));
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are round(y)
+  const float2 t = fadd2(y, make_float2(kRound, kRound));
+  const float2 n = fadd2(t, make_float2(-kRound, -kRound));
+  const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), y);
+  float2 p = ffma2(f, make_float2(0x1.5bd38cp-10f, 0x1.5bd38cp-10f), make_float2(0x1.3cf696p-7f, 0x1.3cf696p-7f));
+  p = ffma2(p, f, make_float2(0x1.c6b740p-5f, 0x1.c6b740p-5f));
+  p = ffma2(p, f, make_float2(0x1.ebf992p-3f, 0x1.ebf992p-3f));
+  p = ffma2(p, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
+  p = ffma2(p, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

@@ -50,32 +50,42 @@ void paged_split_slots(const int* q_lens, const int* kv_lens, size_t n, int head
         range(i, j, &t0, &t1);
         if (t1 > t0) cost += (long long)heads * (t1 - t0 + kFixed);
       }
-  const long long quota = std::max<long long>((cost + slots - 1) / slots, 4 + kFixed);
-  long long left = quota;
-  auto close = [&] {
-    if ((int)out->segs.size() > out->first.back()) out->first.push_back((int)out->segs.size());
-    left = quota;
-  };
-  for (size_t i = 0; i < n; ++i) {
-    if (!chosen(i)) continue;
-    for (int h = 0; h < heads; ++h)
-      for (int j = 0; j < kv_lens[i]; j += kWeightSlots) {
-        int t0, t1;
-        range(i, j, &t0, &t1);
-        const int part0 = out->parts;
-        while (t0 < t1) {
-          if (left - kFixed < std::min(4, t1 - t0) && left < quota) close();
-          int take = (int)std::min<long long>(t1 - t0, std::max<long long>(left - kFixed, 1));
-          if (t1 - t0 - take < 4) take = t1 - t0;
-          out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++});
-          t0 += take;
-          left -= take + kFixed;
-          if (left <= kFixed) close();
+  long long quota = std::max<long long>((cost + slots - 1) / slots, 4 + kFixed);
+  // CTAs that close early may push their count past `slots`, and one CTA more
+  // than the SMs hold costs a whole wave: then with a larger quota
+  for (int attempt = 0;; ++attempt) {
+    out->segs.clear();
+    out->joins.clear();
+    out->first.assign(1, 0);
+    out->parts = 0;
+    long long left = quota;
+    auto close = [&] {
+      if ((int)out->segs.size() > out->first.back()) out->first.push_back((int)out->segs.size());
+      left = quota;
+    };
+    for (size_t i = 0; i < n; ++i) {
+      if (!chosen(i)) continue;
+      for (int h = 0; h < heads; ++h)
+        for (int j = 0; j < kv_lens[i]; j += kWeightSlots) {
+          int t0, t1;
+          range(i, j, &t0, &t1);
+          const int part0 = out->parts;
+          while (t0 < t1) {
+            if (left - kFixed < std::min(4, t1 - t0) && left < quota) close();
+            int take = (int)std::min<long long>(t1 - t0, std::max<long long>(left - kFixed, 1));
+            if (t1 - t0 - take < 4) take = t1 - t0;
+            out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++});
+            t0 += take;
+            left -= take + kFixed;
+            if (left <= kFixed) close();
+          }
+          out->joins.push_back({(int)i, h, j, part0, out->parts - part0});
         }
-        out->joins.push_back({(int)i, h, j, part0, out->parts - part0});
-      }
+    }
+    close();
+    if ((int)out->first.size() - 1 <= slots || attempt == 16) return;
+    quota += std::max<long long>(1, quota / 32);
   }
-  close();
 }
 
 namespace {
@@ -153,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int kv = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
       const int* table = a.s.table + (size_t)g.seq * a.s.stride;
       const int nth = si - seg0, kb = nth & 1;
-      if (nth >= 2 && !mbar_wait_bounded(k_empty + 8 * kb, ((nth >> 1) - 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+      if (nth >= 2 && !mbar_wait(k_empty + 8 * kb, ((nth >> 1) - 1) & 1, abort_flag)) gave_up = true;
       if (__any_sync(0xffffffffu, gave_up)) {
         gave_up = true;
         break;
@@ -173,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int it = g.it0; it < g.it1; ++it, ++n) {
         const int st = n % kStages, round = n / kStages;
-        if (round > 0 && !mbar_wait_bounded(q_empty + 8 * st, (round - 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (round > 0 && !mbar_wait(q_empty + 8 * st, (round - 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
           break;
@@ -191,44 +201,50 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (gave_up) *abort_flag = 1;
   } else if (w == 9) {
     // ---------------- MMAs ----------------
-    if (lane == 0) {
-      int n = 0;
-      auto wait = [&](uint32_t bar, int phase) {
-        if (!gave_up && !mbar_wait_bounded(bar, phase & 1, kWaitNs, abort_flag)) gave_up = true;
-        return !gave_up;
-      };
-      for (int si = seg0; si < seg1 && !gave_up; ++si) {
-        const PagedSeg g = segs[si];
-        const int nth = si - seg0, kb = nth & 1;
-        if (!wait(k_full + 8 * kb, nth >> 1)) break;
-        for (int it = g.it0; it < g.it1; ++it, ++n) {
-          const int st = n % kStages, buf = n & 1;
-          if (!wait(q_full + 8 * st, n / kStages)) break;
+    const bool lead = lane == 0;
+    const uint32_t kd = desc_k(smem(ks)), qd = desc_k(smem(qs));
+    int n = 0, st = 0;
+    uint32_t st_phase = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!mbar_wait(bar, parity, abort_flag)) gave_up = true;
+      if (__any_sync(0xffffffffu, gave_up)) gave_up = true;
+      return !gave_up;
+    };
+    for (int si = uniform(seg0); si < uniform(seg1) && !gave_up; ++si) {
+      const int count = uniform(segs[si].it1 - segs[si].it0);
+      const int nth = si - uniform(seg0), kb = nth & 1;
+      if (!wait(k_full + 8 * kb, (nth >> 1) & 1)) break;
+      for (int it = 0; it < count; ++it, ++n) {
+        const int buf = n & 1;
+        if (!wait(q_full + 8 * st, st_phase)) break;
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            const int b = 2 * kt + buf;
-            if (n >= 2 && !wait(s_empty + 8 * b, (n >> 1) - 1)) break;
-            fence_after();
-            const uint32_t k = smem(ks) + (2 * kb + kt) * kBytes, q = smem(qs) + st * kBytes;
+        for (int kt = 0; kt < 2; ++kt) {
+          const int b = 2 * kt + buf;
+          if (n >= 2 && !gave_up) wait(s_empty + 8 * b, ((n >> 1) - 1) & 1);
+          if (gave_up) continue;
+          fence_after();
+          const uint32_t k = kd + (2 * kb + kt) * (kBytes >> 4), q = qd + st * (kBytes >> 4);
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-              const uint32_t off = (d >> 2) * kHalf + (d & 3) * 32;
-              mma_ss(tmem + b * 128, desc_k(k + off), desc_k(q + off), idesc<T>(kTile, false), d > 0);
-            }
-            commit(s_full + 8 * b);
+          for (int d = 0; d < DP / 16; ++d) {
+            const uint32_t off = ((d >> 2) * kHalf + (d & 3) * 32) >> 4;
+            mma_ss(lead, tmem + b * 128, k + off, q + off, idesc<T>(kTile, false), d > 0);
           }
-          if (gave_up) break;
-          commit(q_empty + 8 * st);
+          commit(lead, s_full + 8 * b);
         }
-        if (!gave_up) commit(k_empty + 8 * kb);
+        if (gave_up) break;
+        commit(lead, q_empty + 8 * st);
+        if (++st == kStages) {
+          st = 0;
+          st_phase ^= 1u;
+        }
       }
-      if (gave_up) {  // the MMAs in flight still use this CTA's memory
-        *abort_flag = 1;
-        commit(drained);
-        mbar_wait_bounded(drained, 0, kWaitNs);
-      }
+      if (!gave_up) commit(lead, k_empty + 8 * kb);
     }
-    __syncwarp();
+    if (gave_up) {  // the MMAs in flight still use this CTA's memory
+      *abort_flag = 1;
+      commit(lead, drained);
+      mbar_wait_bounded(drained, 0, kWaitNs);
+    }
   } else if (w >= 10) {
     // ---------------- lse of the rows ----------------
     const int c0 = (w - 10) * 32 + lane;  // columns c0 and c0 + 64
@@ -248,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             z[u] = a.lse[(size_t)(q0 + t) * Hq + g.head * a.group + c % a.group] * (float)M_LOG2E;
           if (z[u] == -INFINITY) z[u] = INFINITY;
         }
-        if (round > 0 && !mbar_wait_bounded(q_empty + 8 * st, (round - 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (round > 0 && !mbar_wait(q_empty + 8 * st, (round - 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
           break;
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float2 c2 = make_float2(a.scale2, a.scale2);
       for (int it = g.it0; it < g.it1; ++it, ++n) {
         const int st = n % kStages, b = 2 * kt + (n & 1);
-        if (!mbar_wait_bounded(s_full + 8 * b, (n >> 1) & 1, kWaitNs, abort_flag)) gave_up = true;
+        if (!mbar_wait(s_full + 8 * b, (n >> 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
           break;
