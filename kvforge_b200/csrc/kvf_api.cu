@@ -2542,7 +2542,7 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
   if (err == cudaSuccess && decay >= 0.0f && plan->slots_n) {
     err = cudaErrorNotSupported;
     if (plan->weights.joins_n) {
-      float* part_w = sc.get<float>((size_t)plan->weights.parts * kWeightSlots);
+      float* part_w = sc.get<float>((size_t)2 * plan->weights.parts * kWeightSlots);
       err = part_w ? launch_paged_chunk_weights(a, plan->weights, plan->tokens, part_w, decay, st)
                    : cudaErrorMemoryAllocation;
     }

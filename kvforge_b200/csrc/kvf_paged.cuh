@@ -149,7 +149,7 @@ constexpr int kChunkRows = 256, kChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
 
 // their attention weights, from a.lse: up to 128 query heads per KV head;
-// part_w: w.parts * kWeightSlots floats. cudaErrorNotSupported (before any
+// part_w: 2 * w.parts * kWeightSlots floats. cudaErrorNotSupported (before any
 // launch) where the queries' strides or alignment do not suit tensor maps.
 // The work: tiles of kWeightSlots slots by row tiles of 128 / group tokens.
 constexpr int kWeightSlots = 256;

@@ -51,10 +51,6 @@ constexpr int kThreads = 32 * (kSoftmaxWarps + 4);
 // what the others give up: 256 x 200 + 128 x 104 = 384 x 168
 constexpr int kRegsSoftmax = 200, kRegsOther = 104;
 
-// of eight pairs of numerators, how many are computed on the multiply-add units
-// (every other pair is a candidate): the exponential unit alone needs as long as
-// the tensor core
-constexpr int kFmaOf4 = 0;
 // quarter of a tile after which the other row tile may start its own
 constexpr int kHandOver = 0;
 
@@ -466,12 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 y1 = ffma2(make_float2(x[32 * q + 2 * e + 2], x[32 * q + 2 * e + 3]), c2, mu2);
             y0.x = ex2(y0.x);
             y0.y = ex2(y0.y);
-            if ((e / 2) % 4 < kFmaOf4) {
-              y1 = ex2_fma(y1);
-            } else {
-              y1.x = ex2(y1.x);
-              y1.y = ex2(y1.y);
-            }
+            y1.x = ex2(y1.x);
+            y1.y = ex2(y1.y);
             sum0 = fadd2(sum0, y0);
             sum1 = fadd2(sum1, y1);
             // the numerators are rounded to the cache's type for the product

@@ -175,26 +175,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^y of two values on the multiply-add units instead of the exponential unit
-// (16 per cycle and SM): 2^n * 2^f with n = round(y) and f = y - n in [-1/2, 1/2],
-// 2^f = 1 + f q(f) with q of degree 4 fitted for the least relative error by
-// linear programming on 4001 points; off by at most 1.7e-7 in all, as ex2.approx.
-// 0 below 2^-127; NaN is NOT handed on (the callers see to it).
-__device__ __forceinline__ float2 ex2_fma(float2 y) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y.y));
-  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are round(y)
-  const float2 t = fadd2(y, make_float2(kRound, kRound));
-  const float2 n = fadd2(t, make_float2(-kRound, -kRound));
-  const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), y);
-  float2 p = ffma2(f, make_float2(0x1.5bd38cp-10f, 0x1.5bd38cp-10f), make_float2(0x1.3cf696p-7f, 0x1.3cf696p-7f));
-  p = ffma2(p, f, make_float2(0x1.c6b740p-5f, 0x1.c6b740p-5f));
-  p = ffma2(p, f, make_float2(0x1.ebf992p-3f, 0x1.ebf992p-3f));
-  p = ffma2(p, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
-  p = ffma2(p, f, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) {

@@ -10,11 +10,14 @@
 // 32768 exponentials 2048, which bound the kernel. The row tiles are divided
 // over the SMs in equal shares; the parts of a slot are added, in order, and
 // joined with the old weight by a second small kernel.
-//   warps 0-3, 4-7: the sums of the first and the second 128 slots
-//   warp 8: tensor-map loads of K (a box per page; the next segment's while
+//   warps 0-7, 8-15: the sums of the first and the second 128 slots, four warps
+//     for one half of a tile's rows and four for the other (two warps per
+//     scheduler left the exponential unit half idle: 238 instead of 165 us for two
+//     1000-token chunks on 7000 slots)
+//   warp 16: tensor-map loads of K (a box per page; the next segment's while
 //     this one runs) and of the rows (group heads by 128 / group tokens)
-//   warp 9: the MMAs, one thread; two TMEM buffers per 128 slots
-//   warps 10, 11: lse of the tile's rows, +inf for rows that see nothing and
+//   warp 17: the MMAs, issued by one thread; two TMEM buffers per 128 slots
+//   warps 18, 19: lse of the tile's rows, +inf for rows that see nothing and
 //     for padding, whose terms so become 0
 // Every wait is bounded; one that runs out ends all roles and sets kDevErrTimeout.
 #include <algorithm>
@@ -92,7 +95,8 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kThreads = 384;
+constexpr int kSumWarps = 16;
+constexpr int kThreads = 32 * (kSumWarps + 4);
 template <int DP>
 constexpr int tile_bytes() { return kTile * DP * 2; }
 template <int DP>
@@ -118,18 +122,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &sh_abort;
   const uint32_t q_full = smem(bars), q_empty = q_full + 8 * kStages, k_full = q_empty + 8 * kStages,
                  k_empty = k_full + 16, s_full = k_empty + 16, s_empty = s_full + 32, drained = s_empty + 32;
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int TQ = kTile / a.group, cols = TQ * a.group;  // tokens and rows of a row tile
 
-  if (w == 9) {
+  if (w == kSumWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem(&sh_tmem)),
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(q_full + 8 * i, 3);   // the load and warps 10 and 11
-      mbar_init(q_empty + 8 * i, 9);  // the MMAs' completion and the eight summing warps
+      mbar_init(q_full + 8 * i, 3);               // the load and warps 18 and 19
+      mbar_init(q_empty + 8 * i, 1 + kSumWarps);  // the MMAs' completion and the summing warps
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + 8 * i, 1);
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(s_full + 8 * i, 1);
-      mbar_init(s_empty + 8 * i, 4);
+      mbar_init(s_empty + 8 * i, kSumWarps / 2);
     }
     mbar_init(drained, 1);
     sh_abort = 0;
@@ -150,11 +154,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sh_tmem;
+  constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they start at 0
   const int seg0 = __ldg(first + blockIdx.x), seg1 = __ldg(first + blockIdx.x + 1);
   bool gave_up = false;
 
-  if (w == 8) {
+  if (w == kSumWarps) {
     // ---------------- loads ----------------
     const int page = 1 << a.c.page_shift, box = min(kTile, page);
     int n = 0;
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (gave_up) *abort_flag = 1;
-  } else if (w == 9) {
+  } else if (w == kSumWarps + 1) {
     // ---------------- MMAs ----------------
     const bool lead = lane == 0;
     const uint32_t kd = desc_k(smem(ks)), qd = desc_k(smem(qs));
@@ -245,9 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit(lead, drained);
       mbar_wait_bounded(drained, 0, kWaitNs);
     }
-  } else if (w >= 10) {
+  } else if (w > kSumWarps + 1) {
     // ---------------- lse of the rows ----------------
-    const int c0 = (w - 10) * 32 + lane;  // columns c0 and c0 + 64
+    const int c0 = (w - kSumWarps - 2) * 32 + lane;  // columns c0 and c0 + 64
     const int Hq = a.c.heads * a.group;
     int n = 0;
     for (int si = seg0; si < seg1 && !gave_up; ++si) {
@@ -278,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (gave_up) *abort_flag = 1;
   } else {
     // ---------------- sums ----------------
-    const int kt = w >> 2, t = tid & 127;
+    const int kt = w >> 3, half = (w >> 2) & 1, t = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (w & 3)) << 16;
-    int n = 0;
+    int n = 0, st = 0;
     for (int si = seg0; si < seg1 && !gave_up; ++si) {
       const PagedSeg g = segs[si];
       const int kv = __ldg(a.s.kv_len + g.seq);
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
       const float2 c2 = make_float2(a.scale2, a.scale2);
       for (int it = g.it0; it < g.it1; ++it, ++n) {
-        const int st = n % kStages, b = 2 * kt + (n & 1);
+        const int b = 2 * kt + (n & 1);
         if (!mbar_wait(s_full + 8 * b, (n >> 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
@@ -306,39 +310,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           hi = (pos1 - pos0 + 1) * a.group;
           if (a.window && j >= a.sinks) hi = min(hi, max(0, min(j + a.window - pos0, kTile)) * a.group);
         }
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float x[64];
-          tmem_ld32(tmem + lanes + b * 128 + 64 * q, x);
-          tmem_ld32(tmem + lanes + b * 128 + 64 * q + 32, x + 32);
+#pragma unroll 1
+        for (int q = 64 * half; q < 64 * half + 64; q += 32) {
+          float x[32];
+          tmem_ld32(tmem + lanes + b * 128 + q, x);
           tmem_wait_ld();
-          if (q == 1) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty + 8 * b);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 z = *reinterpret_cast<const float4*>(&lse2[st][q + e]);
+            const float2 y0 = ffma2(make_float2(x[e], x[e + 1]), c2, make_float2(-z.x, -z.y));
+            const float2 y1 = ffma2(make_float2(x[e + 2], x[e + 3]), c2, make_float2(-z.z, -z.w));
+            x[e] = y0.x;
+            x[e + 1] = y0.y;
+            x[e + 2] = y1.x;
+            x[e + 3] = y1.y;
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e < lo - q || e >= hi - q) x[e] = -INFINITY;
           }
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            const float4 z = *reinterpret_cast<const float4*>(&lse2[st][64 * q + e]);
-            float2 y0 = ffma2(make_float2(x[e], x[e + 1]), c2, make_float2(-z.x, -z.y));
-            float2 y1 = ffma2(make_float2(x[e + 2], x[e + 3]), c2, make_float2(-z.z, -z.w));
-            if (!whole) {
-              const int c = 64 * q + e;
-              if (c < lo || c >= hi) y0.x = -INFINITY;
-              if (c + 1 < lo || c + 1 >= hi) y0.y = -INFINITY;
-              if (c + 2 < lo || c + 2 >= hi) y1.x = -INFINITY;
-              if (c + 3 < lo || c + 3 >= hi) y1.y = -INFINITY;
-            }
-            sum0.x += ex2(y0.x);
-            sum0.y += ex2(y0.y);
-            sum1.x += ex2(y1.x);
-            sum1.y += ex2(y1.y);
+          for (int e = 0; e < 32; e += 4) {
+            sum0 = fadd2(sum0, make_float2(ex2(x[e]), ex2(x[e + 1])));
+            sum1 = fadd2(sum1, make_float2(ex2(x[e + 2]), ex2(x[e + 3])));
           }
         }
+        fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_empty + 8 * st);
+        if (lane == 0) {
+          mbar_arrive(s_empty + 8 * b);
+          mbar_arrive(q_empty + 8 * st);
+        }
+        if (++st == kStages) st = 0;
       }
-      if (!gave_up) part_w[(size_t)g.part * kWeightSlots + kt * kTile + t] = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      if (!gave_up)
+        part_w[((size_t)g.part * 2 + half) * kWeightSlots + kt * kTile + t] = (sum0.x + sum0.y) + (sum1.x + sum1.y);
     }
     if (gave_up) *abort_flag = 1;
   }
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  if (w == 8 && sh_abort && lane < kStages + 2) {
+  if (w == kSumWarps && sh_abort && lane < kStages + 2) {
     // after a timeout, the loads in flight still land in this CTA's memory: give
     // them the time of one more bounded wait each (their barriers' phases are
     // not known here, so both are waited for)
@@ -354,7 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_wait_bounded(bar, 0, 10000000ull);
     mbar_wait_bounded(bar, 1, 10000000ull);
   }
-  if (w == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  if (w == kSumWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
 // weight = decay * weight + the parts of its slot
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kWeightSlots) k_paged_chunk_weights_join(Paged
   if (j >= __ldg(a.s.kv_len + g.seq)) return;
   float t = 0.0f;
 #pragma unroll 4
-  for (int p = 0; p < g.parts; ++p) t += __ldg(part_w + (size_t)(g.part0 + p) * kWeightSlots + threadIdx.x);
+  for (int p = 0; p < 2 * g.parts; ++p) t += __ldg(part_w + ((size_t)2 * g.part0 + p) * kWeightSlots + threadIdx.x);
   const int page = __ldg(a.s.table + (size_t)g.seq * a.s.stride + (j >> a.c.page_shift));
   float* p = a.c.weights + (((size_t)page * a.c.heads + g.head) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
   *p = decay == 0.0f ? t : fmaf(decay, *p, t);
