@@ -5,10 +5,15 @@
 // once for up to 16 rows, so the kernel is bound by HBM; its products run on
 // mma.sync m16n8k16 with the rows as M (tcgen05's M of 128 would be mostly
 // padding, and the tensor cores are not what limits here). One producer warp
-// keeps tensor-map loads of 64-slot tiles in flight, a box per page; four
-// consumer warps take 16 slots each, with a running maximum and sum of their
-// own, and are joined once per segment. Two CTAs per SM keep about 190 KB of
+// keeps tensor-map loads of 64-slot tiles in flight, a box per page, and puts
+// the rows of the next segment beside them; two CTAs per SM keep about 190 KB of
 // loads in flight, four times what the latency-bandwidth product asks for.
+// Four consumer warps take 16 slots each for the scores, tell each other their
+// maxima, and put the numerators in shared memory; then each takes a quarter of
+// the columns of V over all 64 slots. So a segment ends without joining sums
+// across warps, and short sequences cost little more than their loads (with a
+// running maximum and sums of its own for each warp, joined at the end of every
+// segment, a batch of 64 sequences of 0 to 16383 slots took 256 us).
 //
 // Slots that no row sees are masked by selection, and their values are
 // replaced by zeros in shared memory, whatever the pages hold. A non-finite
@@ -30,9 +35,28 @@ template <int DP>
 constexpr int stages() { return DP == 128 ? 3 : 6; }
 template <int DP>
 constexpr int tile_bytes() { return kKeys * DP * 2; }
+// a segment as the producer hands it to the consumers
+struct Head {
+  int seq, head, row0, it0, it1, part, n, nq, q0;
+};
+constexpr int kPStride = kKeys + 8;  // numerators of a row, 16-bit: eight rows apart lie in different banks
+template <int DP>
+struct Shared {
+  uint16_t q[2][kRows * DP];  // rows of two segments, 16-byte chunks permuted by the row
+  uint16_t p[kRows * kPStride];
+  float m[kWarps][kRows];
+  float l[kWarps][kRows];
+  Head head[2];
+  uint64_t bars[2 * stages<DP>() + 4];
+  // whether a segment's tiles held non-finite values (by the segment's parity:
+  // the other one is cleared meanwhile); whether a consumer gave up waiting for
+  // the segment's rows or for a tile: each is read between the barrier behind
+  // its wait and the next one, so all four stop together
+  int bad[2], stop_rows, stop, abort;
+};
 template <int DP>
 constexpr size_t smem_bytes() {
-  return 1024 + (size_t)stages<DP>() * 2 * tile_bytes<DP>() + kRows * DP * sizeof(float);
+  return 1024 + (size_t)stages<DP>() * 2 * tile_bytes<DP>() + sizeof(Shared<DP>);
 }
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
@@ -73,60 +97,98 @@ __device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
   return (uint32_t)((chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+// the sum of the non-finite values of one column that the query at slot pos
+// sees in 16-slot groups that not every row of the segment sees whole (v: the
+// column in the pool's first row)
+template <typename T>
+__device__ __noinline__ float nonfinite_sum(const T* v, const int* table, int shift, int heads, int head, int dim,
+                                            int it0, int it1, PagedSpan span, int pa, int pb, int pos, int window,
+                                            int sinks) {
+  float sum = 0.0f;
+  for (int it = it0; it < it1; ++it) {
+    const int t0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys;
+    for (int j = t0; j < t0 + kKeys && j <= pos; ++j) {
+      const int b0 = j & ~15;
+      if ((b0 + 15 <= pa && (!window || b0 > pb - window || b0 + 16 <= sinks)) || !paged_sees(pos, j, window, sinks))
+        continue;
+      const size_t row = (((size_t)__ldg(table + (j >> shift)) * heads + head) << shift) + (j & ((1 << shift) - 1));
+      const float y = to_float<T>(v[row * dim]);
+      if (!isfinite(y)) sum += y;
+    }
+  }
+  return sum;
+}
+
 // scores != nullptr: every score (base 2, -inf where unseen) is also written,
 // for the attention weights: sequence i's at scores + score_at[i], [head][row][slot]
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 2)
     k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttn a,
                    const PagedSeg* __restrict__ segs, const int* __restrict__ first, float* __restrict__ scores,
-                   const long long* __restrict__ score_at) {
-  constexpr int kStages = stages<DP>(), kTile = tile_bytes<DP>(), kSteps = DP / 16, kCols = DP / 8;
+                   const long long* __restrict__ score_at, bool wide_q) {
+  constexpr int kStages = stages<DP>(), kTile = tile_bytes<DP>(), kSteps = DP / 16;
+  constexpr int kCols = DP / (8 * kWarps);  // 8-wide column tiles of a warp
   extern __shared__ uint8_t sm_raw[];
   // the 128-byte swizzle takes its pattern from address bits 7-9
   uint8_t* sm = sm_raw + ((1024u - (ptx::smem(sm_raw) & 1023u)) & 1023u);
-  float* merged = reinterpret_cast<float*>(sm + (size_t)kStages * 2 * kTile);  // [kRows][DP]
-  __shared__ uint64_t bars[2 * kStages];
-  __shared__ float sh_m[kWarps][kRows], sh_l[kWarps][kRows];
-  // whether a segment's tiles held non-finite values (by the segment's parity:
-  // the other one is cleared meanwhile), whether its consumers gave up
-  __shared__ int sh_bad[2], sh_stop;
-  __shared__ int sh_abort;
-  volatile int* abort_flag = &sh_abort;
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  const uint32_t full = ptx::smem(bars), empty = ptx::smem(bars + kStages);
+  Shared<DP>& sh = *reinterpret_cast<Shared<DP>*>(sm + (size_t)kStages * 2 * kTile);
+  volatile int* abort_flag = &sh.abort;
+  const int tid = threadIdx.x, w = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const uint32_t full = ptx::smem(sh.bars), empty = full + 8 * kStages, q_full = empty + 8 * kStages,
+                 q_empty = q_full + 16;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       ptx::mbar_init(full + 8 * i, 1);
       ptx::mbar_init(empty + 8 * i, kWarps);
     }
-    sh_abort = sh_stop = sh_bad[0] = sh_bad[1] = 0;
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(q_full + 8 * i, 1);
+      ptx::mbar_init(q_empty + 8 * i, kWarps);
+    }
+    sh.abort = sh.stop_rows = sh.stop = sh.bad[0] = sh.bad[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   const int seg0 = __ldg(first + blockIdx.x), seg1 = __ldg(first + blockIdx.x + 1);
-  const int box = min(kKeys, 1 << a.c.page_shift);  // slots of one load
   bool gave_up = false;
 
   if (w == kWarps) {
     // ---------------- producer: one lane per box of a tile ----------------
-    int n_tile = 0, pending = 0;
+    const int box = min(kKeys, 1 << a.c.page_shift);  // slots of one load
+    int n_tile = 0;
+    auto describe = [&](int si) {
+      Head d{};
+      if (si < seg1) {
+        const PagedSeg g = segs[si];
+        const int q0 = __ldg(a.s.q_start + g.seq);
+        d = {g.seq, g.head, g.row0, g.it0, g.it1, g.part, __ldg(a.s.kv_len + g.seq),
+             __ldg(a.s.q_start + g.seq + 1) - q0, q0};
+      }
+      return d;
+    };
+    Head next = describe(seg0);
     for (int si = seg0; si < seg1 && !gave_up; ++si) {
-      const PagedSeg g = segs[si];
-      const int n = __ldg(a.s.kv_len + g.seq);
-      const int nq = __ldg(a.s.q_start + g.seq + 1) - __ldg(a.s.q_start + g.seq);
+      const Head g = next;
+      next = describe(si + 1);  // in flight while this segment is loaded
+      const int nth = si - seg0, qb = nth & 1;
+      if (nth >= 2 && !ptx::mbar_wait(q_empty + 8 * qb, ((nth >> 1) - 1) & 1, abort_flag)) gave_up = true;
+      if (__any_sync(0xffffffffu, gave_up)) {
+        gave_up = true;
+        break;
+      }
       const int* table = a.s.table + (size_t)g.seq * a.s.stride;
-      const PagedSpan span = paged_span(g.row0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
-      for (int it = g.it0; it < g.it1; ++it, ++n_tile) {
+      const PagedSpan span = paged_span(g.row0, kRows, a.group, g.n, g.nq, a.window, a.sinks, kKeys);
+      auto load = [&](int it) {
         const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys;
         const int j = j0 + lane * box;
-        const bool mine = lane * box < kKeys && j < n;
+        const bool mine = lane * box < kKeys && j < g.n;
         const int page = mine ? __ldg(table + (j >> a.c.page_shift)) : 0;
         const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
         const int s = n_tile % kStages, round = n_tile / kStages;
         if (round > 0 && !ptx::mbar_wait(empty + 8 * s, (round - 1) & 1, abort_flag)) gave_up = true;
         if (__any_sync(0xffffffffu, gave_up)) {
           gave_up = true;
-          break;
+          return;
         }
         if (lane == 0) ptx::mbar_expect(full + 8 * s, (uint32_t)(boxes * 2 * box * DP * 2));
         __syncwarp();
@@ -139,63 +201,85 @@ __global__ void __launch_bounds__(kThreads, 2)
             ptx::load_box(dst + kTile + half * (kKeys * 128), &vmap, 64 * half, y, z, full + 8 * s);
           }
         }
-        pending = n_tile + 1;
+        ++n_tile;
+      };
+      if (g.it0 < g.it1) load(g.it0);  // ahead of the rows: it takes longer
+      // the segment's rows, rows and columns that are not there as zeros
+      const int rows = min(kRows, g.nq * a.group - g.row0);
+#pragma unroll 4
+      for (int i = lane; i < kRows * (DP / 8); i += 32) {
+        const int r = i / (DP / 8), ch = i - r * (DP / 8);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && 8 * ch < a.c.dim) {
+          const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+          const uint16_t* p =
+              static_cast<const uint16_t*>(a.q) + (size_t)(g.q0 + t) * a.q_token + (size_t)hq * a.q_head + 8 * ch;
+          if (wide_q) x = __ldg(reinterpret_cast<const uint4*>(p));
+          else
+            x = make_uint4(__ldg(p) | ((uint32_t)__ldg(p + 1) << 16), __ldg(p + 2) | ((uint32_t)__ldg(p + 3) << 16),
+                           __ldg(p + 4) | ((uint32_t)__ldg(p + 5) << 16), __ldg(p + 6) | ((uint32_t)__ldg(p + 7) << 16));
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(sh.q[qb]) + r * (DP * 2) + ((ch ^ (r & 7)) << 4)) = x;
       }
+      if (lane == 0) sh.head[qb] = g;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(q_full + 8 * qb);
+      for (int it = g.it0 + 1; it < g.it1 && !gave_up; ++it) load(it);
     }
     // after a timeout the loads in flight still land in this CTA's memory
     if (gave_up) {
       *abort_flag = 1;
-      for (int t = max(0, pending - kStages); t < pending; ++t)
+      for (int t = max(0, n_tile - kStages); t < n_tile; ++t)
         mbar_wait_bounded(full + 8 * (t % kStages), (t / kStages) & 1, kWaitNs);
     }
   } else {
     // ---------------- consumers ----------------
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;  // rows r0, r0 + 8; columns c0, c0 + 1 of an 8-wide tile
     const int Hq = a.c.heads * a.group, D = a.c.dim;
-    int n_tile = 0;
+    int s = 0;
+    uint32_t s_phase = 0;
     for (int si = seg0; si < seg1; ++si) {
-      const PagedSeg g = segs[si];
-      const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
-      const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = min(kRows, nq * a.group - g.row0);
-      const PagedSpan span = paged_span(g.row0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
+      const int nth = si - seg0, qb = nth & 1;
+      if (!ptx::mbar_wait(q_full + 8 * qb, (nth >> 1) & 1, abort_flag)) gave_up = true;
+      if (__any_sync(0xffffffffu, gave_up)) {
+        gave_up = true;
+        *abort_flag = 1;
+        sh.stop_rows = 1;
+      }
+      const Head g = sh.head[qb];
       uint32_t qf[kSteps][4];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        // matrices: rows 0-7 and 8-15 of columns 0-7, then of columns 8-15
+        const int r = lane & 15, ch = 2 * k + (lane >> 4);
+        ldsm4(ptx::smem(sh.q[qb]) + r * (DP * 2) + ((ch ^ (r & 7)) << 4), qf[k]);
+      }
+      consumer_sync();  // also: the last segment's maxima and sums are read
+      if (sh.stop_rows) break;
+      if (tid == 0) sh.bad[(si + 1) & 1] = 0;
+      if (lane == 0) ptx::mbar_arrive(q_empty + 8 * qb);
+      const int rows = min(kRows, g.nq * a.group - g.row0);
+      const PagedSpan span = paged_span(g.row0, kRows, a.group, g.n, g.nq, a.window, a.sinks, kKeys);
       int pos[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = r0 + 8 * i;
-        const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
-        pos[i] = n - nq + t;
-        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
-        const bool pair = (reinterpret_cast<uintptr_t>(p) & 3) == 0;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 16 * k + 8 * e + c0;
-            uint32_t x = 0;
-            if (r < rows && c < D) {  // D is even
-              if (pair) x = __ldg(reinterpret_cast<const uint32_t*>(p + c));
-              else x = (uint32_t)__ldg(p + c) | ((uint32_t)__ldg(p + c + 1) << 16);
-            }
-            qf[k][2 * e + i] = x;
-          }
-      }
-      const int pa = n - nq + g.row0 / a.group, pb = n - nq + (g.row0 + rows - 1) / a.group;
+      for (int i = 0; i < 2; ++i) pos[i] = g.n - g.nq + (g.row0 + r0 + 8 * i) / a.group;
+      const int pa = g.n - g.nq + g.row0 / a.group, pb = g.n - g.nq + (g.row0 + rows - 1) / a.group;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kCols][4];
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
-      float* sc = scores ? scores + score_at[g.seq] + ((size_t)g.head * nq * a.group + g.row0) * n : nullptr;
+      float* sc = scores ? scores + score_at[g.seq] + ((size_t)g.head * g.nq * a.group + g.row0) * g.n : nullptr;
+      bool stop = false;
 
-      for (int it = g.it0; it < g.it1; ++it, ++n_tile) {
-        const int s = n_tile % kStages;
+      for (int it = g.it0; it < g.it1; ++it) {
         const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys + 16 * w;  // this warp's slots
         const uint32_t kt = ptx::smem(sm) + (uint32_t)(s * 2 * kTile), vt = kt + kTile;
-        if (!ptx::mbar_wait(full + 8 * s, (n_tile / kStages) & 1, abort_flag)) gave_up = true;
-        if (__any_sync(0xffffffffu, gave_up)) {
+        if (!ptx::mbar_wait(full + 8 * s, s_phase, abort_flag)) gave_up = true;
+        if (__any_sync(0xffffffffu, gave_up)) {  // all four stop at the next barrier
           gave_up = true;
-          break;
+          *abort_flag = 1;
+          sh.stop = 1;
         }
         float x[2][4] = {};
         {
@@ -210,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         // slots that every row sees need no masks
         const bool whole = j0 + 15 <= pa && (!a.window || j0 > pb - a.window || j0 + 16 <= a.sinks);
-        float mx[2] = {m[0], m[1]};
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -225,49 +309,21 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = r0 + 8 * (e >> 1), j = j0 + 8 * t + c0 + (e & 1);
-              if (r < rows && j < n) sc[(size_t)r * n + j] = x[t][e];
+              if (r < rows && j < g.n) sc[(size_t)r * g.n + j] = x[t][e];
             }
         }
-        float f[2], mu[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
           mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-          mu[i] = mx[i] == -INFINITY ? 0.0f : mx[i];
-          f[i] = ex2(m[i] - mu[i]);
+          if ((lane & 3) == 0) sh.m[w][r0 + 8 * i] = mx[i];
         }
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            l[i] *= f[i];
-            m[i] = mx[i];
-          }
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            o[c][0] *= f[0];
-            o[c][1] *= f[0];
-            o[c][2] *= f[1];
-            o[c][3] *= f[1];
-          }
-        }
-        float p[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[t][e] = ex2(x[t][e] - mu[e >> 1]);
-            l[e >> 1] += p[t][e];
-          }
-        // the numerators are rounded to the cache's type for the product with
-        // the values; the sum keeps them in f32
-        const uint32_t pf[4] = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]),
-                                pack2<T>(p[1][2], p[1][3])};
         if (!whole) {  // this warp's 16 rows of V, two lanes a row
           const int row = lane >> 1, j = j0 + row;
           const bool any = j <= pb && (!a.window || j > pa - a.window || j < a.sinks);
           bool bad = false;
 #pragma unroll 1
-          for (int c = lane & 1; c < kCols; c += 2) {
+          for (int c = lane & 1; c < DP / 8; c += 2) {
             uint4* q = reinterpret_cast<uint4*>(sm + (size_t)s * 2 * kTile + kTile + tile_off(16 * w + row, c));
             if (!any) *q = make_uint4(0, 0, 0, 0);
             else {
@@ -278,101 +334,107 @@ __global__ void __launch_bounds__(kThreads, 2)
               }
             }
           }
-          if (bad) sh_bad[si & 1] = 1;
-          __syncwarp();
+          if (bad) sh.bad[si & 1] = 1;
         }
-        {
-          const int row = 16 * w + (lane & 15), odd = lane >> 4;
+        consumer_sync();  // the maxima are there
+        if (sh.stop) {
+          stop = true;
+          break;
+        }
+        float f[2], mu[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float M = m[i];
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) M = fmaxf(M, sh.m[k][r0 + 8 * i]);
+          mu[i] = M == -INFINITY ? 0.0f : M;
+          f[i] = ex2(m[i] - mu[i]);
+          l[i] *= f[i];
+          m[i] = M;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[t][e] = ex2(x[t][e] - mu[e >> 1]);
+            l[e >> 1] += x[t][e];
+          }
+          // the numerators are rounded to the cache's type for the product with
+          // the values; the sum keeps them in f32
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint32_t*>(&sh.p[(r0 + 8 * i) * kPStride + 16 * w + 8 * t + c0]) =
+                pack2<T>(x[t][2 * i], x[t][2 * i + 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          o[c][0] *= f[0];
+          o[c][1] *= f[0];
+          o[c][2] *= f[1];
+          o[c][3] *= f[1];
+        }
+        consumer_sync();  // the numerators (and V, put right) are there
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+          uint32_t pf[4];
+          ldsm4(ptx::smem(sh.p) + ((lane & 15) * kPStride + 16 * k + 8 * (lane >> 4)) * 2, pf);
 #pragma unroll
           for (int c = 0; c < kCols; c += 2) {
             uint32_t b[4];
-            ldsm4t(vt + tile_off(row, c + odd), b);
+            ldsm4t(vt + tile_off(16 * k + (lane & 15), kCols * w + c + (lane >> 4)), b);
             mma16816<T>(o[c], pf, b[0], b[1]);
             mma16816<T>(o[c + 1], pf, b[2], b[3]);
           }
         }
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(empty + 8 * s);
+        if (++s == kStages) {
+          s = 0;
+          s_phase ^= 1u;
+        }
       }
-      if (gave_up) {  // the other warps' waits end by it too
-        *abort_flag = 1;
-        sh_stop = 1;
-      }
-      // join the four warps: row maxima first, then the rescaled sums in order
+      if (stop) break;
+      // every warp knows the rows' maxima; their sums are added up
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if ((lane & 3) == 0) {
-          sh_m[w][r0 + 8 * i] = m[i];
-          sh_l[w][r0 + 8 * i] = l[i];
-        }
+        if ((lane & 3) == 0) sh.l[w][r0 + 8 * i] = l[i];
       }
       consumer_sync();
-      if (tid == 0) sh_bad[(si + 1) & 1] = 0;
-      float f[2];
+      const bool bad = sh.bad[si & 1] != 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float M = sh_m[0][r0 + 8 * i];
+        const int r = r0 + 8 * i;
+        if (r >= rows) continue;
+        float L = sh.l[0][r];
 #pragma unroll
-        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sh_m[k][r0 + 8 * i]);
-        f[i] = M == -INFINITY ? 0.0f : ex2(m[i] - M);
-      }
-      for (int k = 0; k < kWarps; ++k) {
-        if (w == k) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float2* q = reinterpret_cast<float2*>(merged + (r0 + 8 * i) * DP + 8 * c + c0);
-              float2 v = k ? *q : make_float2(0.0f, 0.0f);
-              v.x += o[c][2 * i] * f[i];
-              v.y += o[c][2 * i + 1] * f[i];
-              *q = v;
-            }
-        }
-        consumer_sync();
-      }
-      // read between two barriers, so that all warps go on or stop together
-      const bool bad = sh_bad[si & 1] != 0, stop = sh_stop != 0;
-      for (int i = tid; i < rows * DP; i += 32 * kWarps) {
-        const int r = i / DP, c = i - r * DP;
-        if (c >= D) continue;
-        float M = sh_m[0][r], L = 0.0f, v = merged[i];
-#pragma unroll
-        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sh_m[k][r]);
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) L += M == -INFINITY ? 0.0f : sh_l[k][r] * ex2(sh_m[k][r] - M);
+        for (int k = 1; k < kWarps; ++k) L += sh.l[k][r];
         const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
-        if (bad) {  // non-finite values that were taken out of tiles that not every row sees whole
-          const int* table = a.s.table + (size_t)g.seq * a.s.stride;
-          for (int it = g.it0; it < g.it1; ++it) {
-            const int t0 = (it < span.nsink ? it : span.first + it - span.nsink) * kKeys;
-            for (int j = t0; j < t0 + kKeys && j <= n - nq + t; ++j) {
-              const int b0 = j & ~15;
-              if ((b0 + 15 <= pa && (!a.window || b0 > pb - a.window || b0 + 16 <= a.sinks)) ||
-                  !paged_sees(n - nq + t, j, a.window, a.sinks))
-                continue;
-              const float y = to_float<T>(static_cast<const T*>(a.c.values)[paged_row(table, a.c, g.head, j) + c]);
-              if (!isfinite(y)) v += y;
-            }
+        const size_t at = (size_t)(g.q0 + t) * Hq + hq;
+        const bool none = L == 0.0f;
+        const float inv = none ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = 8 * (kCols * w + c) + c0 + e;
+            if (col >= D) continue;
+            float v = o[c][2 * i + e];
+            if (bad)
+              v += nonfinite_sum<T>(static_cast<const T*>(a.c.values) + col, a.s.table + (size_t)g.seq * a.s.stride,
+                                    a.c.page_shift, a.c.heads, g.head, D, g.it0, g.it1, span, pa, pb, g.n - g.nq + t,
+                                    a.window, a.sinks);
+            if (g.part >= 0) a.part_o[((size_t)g.part * kRows + r) * D + col] = v;
+            else static_cast<T*>(a.out)[at * D + col] = from_float<T>(none ? 0.0f : v * inv);
           }
-        }
-        const size_t at = (size_t)(q0 + t) * Hq + hq;
-        if (g.part >= 0) {
-          a.part_o[((size_t)g.part * kRows + r) * D + c] = v;
-          if (c == 0) {
-            a.part_ml[((size_t)g.part * kRows + r) * 2] = M;
-            a.part_ml[((size_t)g.part * kRows + r) * 2 + 1] = L;
-          }
-        } else {
-          const bool none = L == 0.0f;
-          static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : v / L);
-          if (c == 0 && a.lse) a.lse[at] = none ? -INFINITY : (M + log2f(L)) * (float)M_LN2;
+        if (w == 0 && (lane & 3) == 0) {
+          if (g.part >= 0)
+            *reinterpret_cast<float2*>(a.part_ml + ((size_t)g.part * kRows + r) * 2) = make_float2(m[i], L);
+          else if (a.lse)
+            a.lse[at] = none ? -INFINITY : (m[i] + log2f(L)) * (float)M_LN2;
         }
       }
-      consumer_sync();  // the joined sums are read before the next segment writes them
-      if (stop) break;
     }
   }
   if (gave_up && a.status) atomicOr(a.status, kDevErrTimeout);
@@ -422,7 +484,8 @@ cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& vm, const Pag
   constexpr size_t smem = smem_bytes<DP>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  kern<<<w.ctas, kThreads, smem, st>>>(km, vm, a, w.segs, w.first, scores, score_at);
+  const bool wide_q = (a.q_token | a.q_head) % 8 == 0 && aligned(a.q, 16);
+  kern<<<w.ctas, kThreads, smem, st>>>(km, vm, a, w.segs, w.first, scores, score_at, wide_q);
   note_launches(1);
   return cudaGetLastError();
 }
