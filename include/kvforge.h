@@ -429,10 +429,11 @@ typedef struct {
  * sequence may have more queries than slots: its first queries then lie before
  * slot 0 and see nothing. Every page that the lengths reach is checked against
  * num_pages; the arrays are read before the call returns. The plan copies them
- * to the device on `stream` and may be used on any stream; on another one its
- * calls first wait for that copy. kvf_paged_plan_free returns its memory after
- * the last call issued with it on every stream; `stream` and the context must
- * outlive it. */
+ * to the device on `stream`, keeps the attention's workspace, and may be used on
+ * any stream, by one host thread at a time: its calls run one after another on
+ * the GPU, also when they are issued on different streams. kvf_paged_plan_free
+ * returns its memory after the last call issued with it on every stream;
+ * `stream` and the context must outlive it. */
 kvf_status kvf_paged_plan_create(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs,
                                  const int32_t* query_lens_host, const int32_t* kv_lens_host,
                                  const int32_t* page_table_host, size_t table_stride, size_t query_heads,
@@ -446,10 +447,11 @@ kvf_status kvf_paged_append(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_
                             const void* keys, size_t k_token_stride, size_t k_head_stride, const void* values,
                             size_t v_token_stride, size_t v_head_stride, void* stream);
 
-/* Copies one sequence of one layer out of its pages: keys and values
- * [num_heads, kv_len, head_dim] of the pool's dtype, the codec's layout. */
-kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
-                            size_t seq, void* keys, void* values, void* stream);
+/* Copies one sequence of `len` slots of one layer out of its pages
+ * (pages_host: their list, read before the call returns): keys and values
+ * [num_heads, len, head_dim] of the pool's dtype, the codec's layout. */
+kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t layer, const int32_t* pages_host,
+                            size_t len, void* keys, void* values, void* stream);
 
 /* Attention of the plan's new tokens (already in the cache) over one layer:
  *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j   over the slots j that t sees,
@@ -470,18 +472,20 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
                                const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
                                float decay, void* out, float* lse, void* stream);
 
-/* Keeps `budget` slots of every sequence of the plan, for each layer and KV
- * head on its own: the first `sinks`, the last `recent`, and of the others
- * those with the largest weight (among equals the lowest slot; NaN counts
- * below every number). The kept slots' keys, values and weights are copied, in
- * order, into the pages of new_table_host [num_seqs, new_table_stride], which
- * must be disjoint from the plan's; the sources stay as they are. A sequence
- * of at most `budget` slots keeps them all. kept (device) [num_layers,
- * num_seqs, num_heads, budget] i32: the slots, -1 behind the last.
- * KVF_ERR_INVALID_CONFIG when sinks + recent > budget. */
-kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t budget,
-                           size_t recent, size_t sinks, const int32_t* new_table_host, size_t new_table_stride,
-                           int32_t* kept, void* stream);
+/* Keeps `budget` slots of every sequence (kv_lens_host[i] slots in the pages of
+ * row i of page_table_host), for each layer and KV head on its own: the first
+ * `sinks`, the last `recent`, and of the others those with the largest weight
+ * (among equals the lowest slot; NaN counts below every number). The kept slots'
+ * keys, values and weights are copied, in order, into the pages of
+ * new_table_host [num_seqs, new_table_stride], which must not be among the
+ * sources' or named twice; the sources stay as they are. A sequence of at most
+ * `budget` slots keeps them all. kept (device) [num_layers, num_seqs, num_heads,
+ * budget] i32: the slots, -1 behind the last. The host arrays are read before
+ * the call returns. KVF_ERR_INVALID_CONFIG when sinks + recent > budget. */
+kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs, const int32_t* kv_lens_host,
+                           const int32_t* page_table_host, size_t table_stride, size_t budget, size_t recent,
+                           size_t sinks, const int32_t* new_table_host, size_t new_table_stride, int32_t* kept,
+                           void* stream);
 
 /* ---- cost model with measured GPU costs (CostModel, crates/kvforge-core/src/cost.rs;
  *      the reference's CpuCostModel is a fixed table, crates/kvforge-cpu/src/cost.rs:9-115)

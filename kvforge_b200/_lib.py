@@ -191,9 +191,9 @@ def _declare(L):
         "kvf_paged_plan_create": (st, [p, C.POINTER(PagedPool), sz, p, p, p, sz, sz, i32, i32, C.POINTER(p), p]),
         "kvf_paged_plan_free": (st, [p]),
         "kvf_paged_append": (st, [p, p, C.POINTER(PagedPool), sz, p, sz, sz, p, sz, sz, p]),
-        "kvf_paged_gather": (st, [p, p, C.POINTER(PagedPool), sz, sz, p, p, p]),
+        "kvf_paged_gather": (st, [p, C.POINTER(PagedPool), sz, p, sz, p, p, p]),
         "kvf_paged_attention": (st, [p, p, C.POINTER(PagedPool), sz, p, sz, sz, C.c_float, C.c_float, p, p, p]),
-        "kvf_paged_evict": (st, [p, p, C.POINTER(PagedPool), sz, sz, sz, p, sz, p, p]),
+        "kvf_paged_evict": (st, [p, C.POINTER(PagedPool), sz, p, p, sz, sz, sz, sz, p, sz, p, p]),
         "kvf_launch_count": (C.c_uint64, []),
         "kvf_stage_name": (C.c_char_p, [i32]),
         "kvf_profile_enable": (st, [p, C.c_int]),

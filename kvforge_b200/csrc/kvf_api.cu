@@ -994,10 +994,9 @@ struct kvf_paged_plan {
   size_t num_pages = 0, heads = 0, dim = 0;
   size_t tokens = 0, group = 0;
   int window = 0, sinks = 0;
-  std::vector<int> kv_lens, q_lens, pages;  // pages: every page in use, sequence after sequence
-  std::vector<size_t> page_start;           // [n + 1] into pages
   void* block = nullptr;  // device: tables and work lists
   PagedSeqs seqs;
+  const long long* place = nullptr;  // [tokens] page and row of every new token
   std::vector<PagedWork> works;
   // tiles of slots whose weights change: of sequences that the CUDA-core
   // kernel sums, and of those whose scores k_paged_decode keeps
@@ -1008,9 +1007,17 @@ struct kvf_paged_plan {
   PagedWork weights;  // the same sequences as `slots`, for the tensor-core sums (joins_n 0: none)
   const long long* score_at = nullptr;  // [n] where a sequence's scores start
   size_t scores_n = 0;
-  cudaEvent_t ready = nullptr;
+  // workspace: parts of cut tiles (for the largest work list) and their
+  // counters; with weights also the scores, the sums' parts, and the rows' lse
+  float* part_o = nullptr;
+  float* part_ml = nullptr;
+  unsigned* counters = nullptr;
+  mutable float* scores = nullptr;
+  mutable float* part_w = nullptr;
+  mutable float* lse = nullptr;
+  mutable cudaStream_t last = nullptr;  // the stream of the last call
   mutable std::mutex use_mu;
-  mutable std::vector<std::pair<cudaStream_t, cudaEvent_t>> uses;
+  mutable std::vector<std::pair<cudaStream_t, cudaEvent_t>> uses;  // last use on every other stream
 };
 
 namespace {
@@ -1091,10 +1098,35 @@ kvf_status upload(kvf_ctx* ctx, void* dst, const void* src, size_t bytes, cudaSt
   return KVF_OK;
 }
 
+// every call of a plan runs behind the one before it: they share its workspace
+kvf_status plan_enter(const kvf_paged_plan* p, cudaStream_t st) {
+  if (st == p->last) return KVF_OK;
+  if (p->last == p->stream) {
+    cudaEvent_t ev = nullptr;
+    KVF_CUDA(p->ctx->order_event(&ev));
+    cudaError_t e = cudaEventRecord(ev, p->stream);
+    if (e == cudaSuccess) e = cudaStreamWaitEvent(st, ev, 0);
+    p->ctx->order_event_release(ev);
+    KVF_CUDA(e);
+  } else {
+    for (auto& u : p->uses)
+      if (u.first == p->last) KVF_CUDA(cudaStreamWaitEvent(st, u.second, 0));
+  }
+  p->last = st;
+  return KVF_OK;
+}
+
+// the plan's workspace of `n` floats, allocated on first use
+kvf_status plan_floats(const kvf_paged_plan* p, float** at, size_t n, cudaStream_t st) {
+  if (!*at)
+    KVF_CUDA(cudaMallocFromPoolAsync(reinterpret_cast<void**>(at), std::max<size_t>(n, 1) * sizeof(float),
+                                     p->ctx->pool, st));
+  return KVF_OK;
+}
+
 kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, const int32_t* kv_lens,
                            const int32_t* table, size_t stride, size_t query_heads) {
   size_t tokens = 0, max_pages = 1, max_kv = 0;
-  p->page_start.assign(1, 0);
   for (size_t i = 0; i < n; ++i) {
     if (q_lens[i] < 0 || kv_lens[i] < 0 || (size_t)kv_lens[i] > kMaxLen || (size_t)q_lens[i] > kMaxLen)
       return fail(KVF_ERR_SHAPE_MISMATCH, "sequence lengths must be in 0..2^30");
@@ -1105,27 +1137,28 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     for (size_t k = 0; k < pages; ++k) {
       const int32_t id = table[i * stride + k];
       if (id < 0 || (size_t)id >= p->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
-      p->pages.push_back(id);
     }
-    p->page_start.push_back(p->pages.size());
     max_pages = std::max(max_pages, pages);
   }
   if (tokens > kMaxLen) return fail(KVF_ERR_SHAPE_MISMATCH, "more than 2^30 new tokens");
   if (tokens * p->group > kMaxLen) return fail(KVF_ERR_SHAPE_MISMATCH, "more than 2^30 query rows per KV head");
   p->tokens = tokens;
-  p->kv_lens.assign(kv_lens, kv_lens + n);
-  p->q_lens.assign(q_lens, q_lens + n);
   // a window or sinks that reach over every slot hide nothing
   if ((size_t)p->window >= max_kv || (size_t)p->sinks >= max_kv) p->window = p->sinks = 0;
 
   BlockImage img;
   std::vector<int> tab(n * max_pages, 0), q_start(n + 1, 0);
+  std::vector<long long> place;
+  place.reserve(tokens);
   for (size_t i = 0; i < n; ++i) {
-    std::copy(p->pages.begin() + p->page_start[i], p->pages.begin() + p->page_start[i + 1],
-              tab.begin() + i * max_pages);
+    const int32_t* pages = table + i * stride;
+    std::copy(pages, pages + ((size_t)kv_lens[i] + p->page_size - 1) / p->page_size, tab.begin() + i * max_pages);
     q_start[i + 1] = q_start[i] + q_lens[i];
+    for (int j = kv_lens[i] - q_lens[i]; j < kv_lens[i]; ++j)
+      place.push_back(j < 0 ? -1 : (long long)pages[j / p->page_size] * 128 + j % p->page_size);
   }
-  const size_t at_table = img.add(tab), at_kv = img.add(p->kv_lens), at_q = img.add(q_start);
+  const size_t at_table = img.add(tab), at_kv = img.add(kv_lens, n), at_q = img.add(q_start),
+               at_place = img.add(place);
 
   struct Offsets { size_t segs, first, joins; };
   std::vector<Offsets> at;
@@ -1141,9 +1174,9 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     const long long few = kDecodeRows;
     static_assert(kDecodeRows == kGenRowsShort, "the same sequences have few rows for both kernels");
     if (tc) {
-      // two CTAs per SM
+      // two CTAs per SM; a segment's start and end cost about five tiles of loads
       hosts[0].kernel = kPagedDecode;
-      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kDecodeRows, kDecodeKeys, 2 * sms, 2, 1,
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kDecodeRows, kDecodeKeys, 2 * sms, 2, 5,
                   &hosts[0]);
     } else {
       paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1,
@@ -1176,11 +1209,25 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     }
     for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});
   }
+  size_t parts_floats = 0, parts_rows = 0, joins = 0;
+  for (size_t i = 0; i < hosts.size() && i < 2; ++i) {
+    parts_rows = std::max(parts_rows, (size_t)hosts[i].parts * hosts[i].row_tile);
+    parts_floats = parts_rows * p->dim;
+    joins = std::max(joins, hosts[i].joins.size());
+  }
+  const std::vector<unsigned> zeros(joins * kJoinCounters, 0u);
+  const size_t at_counters = img.add(zeros);
   const size_t at_slots = img.add(slots), at_decode_slots = img.add(decode_slots), at_score_at = img.add(score_at);
 
-  KVF_CUDA(cudaMallocFromPoolAsync(&p->block, img.bytes.size(), p->ctx->pool, p->stream));
+  // one allocation: the image, then the workspace of the parts
+  const size_t at_ml = align_up(img.bytes.size(), 256), at_o = align_up(at_ml + parts_rows * 2 * sizeof(float), 256);
+  KVF_CUDA(cudaMallocFromPoolAsync(&p->block, at_o + parts_floats * sizeof(float), p->ctx->pool, p->stream));
   KVF_TRY(upload(p->ctx, p->block, img.bytes.data(), img.bytes.size(), p->stream));
   char* d = static_cast<char*>(p->block);
+  p->part_ml = reinterpret_cast<float*>(d + at_ml);
+  p->part_o = reinterpret_cast<float*>(d + at_o);
+  p->counters = reinterpret_cast<unsigned*>(d + at_counters);
+  p->place = reinterpret_cast<const long long*>(d + at_place);
   p->seqs.table = reinterpret_cast<const int*>(d + at_table);
   p->seqs.stride = max_pages;
   p->seqs.kv_len = reinterpret_cast<const int*>(d + at_kv);
@@ -1208,8 +1255,7 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   p->decode_slots = reinterpret_cast<const PagedSlots*>(d + at_decode_slots);
   p->decode_slots_n = decode_slots.size();
   p->score_at = reinterpret_cast<const long long*>(d + at_score_at);
-  KVF_CUDA(p->ctx->order_event(&p->ready));
-  KVF_CUDA(cudaEventRecord(p->ready, p->stream));
+  p->last = p->stream;
   return KVF_OK;
 }
 
@@ -2447,8 +2493,8 @@ kvf_status kvf_paged_plan_free(kvf_paged_plan* plan) {
       cudaStreamWaitEvent(plan->stream, u.second, 0);
       plan->ctx->order_event_release(u.second);
     }
-    if (plan->ready) plan->ctx->order_event_release(plan->ready);
-    if (plan->block) cudaFreeAsync(plan->block, plan->stream);
+    for (void* p : {plan->block, (void*)plan->scores, (void*)plan->part_w, (void*)plan->lse})
+      if (p) cudaFreeAsync(p, plan->stream);
   }
   delete plan;
   return KVF_OK;
@@ -2464,26 +2510,28 @@ kvf_status kvf_paged_append(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_
   if (!aligned(keys, e) || !aligned(values, e)) return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
   DeviceGuard g(ctx->device);
   cudaStream_t st = S(stream);
-  KVF_TRY(reader_enter(plan, st));
-  KVF_CUDA(launch_paged_append(plan->seqs, paged_layer(pool, layer), plan->tokens, keys, k_token_stride, k_head_stride,
+  KVF_TRY(plan_enter(plan, st));
+  KVF_CUDA(launch_paged_append(plan->place, paged_layer(pool, layer), plan->tokens, keys, k_token_stride, k_head_stride,
                                values, v_token_stride, v_head_stride, st));
   return reader_leave(plan, st);
 }
 
-kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
-                            size_t seq, void* keys, void* values, void* stream) {
-  KVF_TRY(check_plan(ctx, plan, pool, layer));
-  if (seq >= plan->kv_lens.size()) return fail(KVF_ERR_SHAPE_MISMATCH, "sequence outside the plan");
-  const size_t len = (size_t)plan->kv_lens[seq];
+kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t layer, const int32_t* pages_host,
+                            size_t len, void* keys, void* values, void* stream) {
+  KVF_TRY(check_ctx(ctx));
+  KVF_TRY(check_pool(pool));
+  if (layer >= pool->num_layers) return fail(KVF_ERR_SHAPE_MISMATCH, "layer outside the pool");
+  if (len > kMaxLen) return fail(KVF_ERR_SHAPE_MISMATCH, "sequence lengths must be in 0..2^30");
   if (len == 0) return KVF_OK;
-  if (!keys || !values) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
-  const size_t e = plan->dtype == KVF_IN_F32 ? 4 : 2;
+  if (!pages_host || !keys || !values) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  for (size_t k = 0; k < (len + pool->page_size - 1) / pool->page_size; ++k)
+    if (pages_host[k] < 0 || (size_t)pages_host[k] >= pool->num_pages)
+      return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
+  const size_t e = pool->dtype == KVF_IN_F32 ? 4 : 2;
   if (!aligned(keys, e) || !aligned(values, e)) return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
   DeviceGuard g(ctx->device);
-  cudaStream_t st = S(stream);
-  KVF_TRY(reader_enter(plan, st));
-  KVF_CUDA(launch_paged_gather(plan->seqs, paged_layer(pool, layer), seq, len, keys, values, st));
-  return reader_leave(plan, st);
+  KVF_CUDA(launch_paged_gather(pages_host, paged_layer(pool, layer), len, keys, values, S(stream)));
+  return KVF_OK;
 }
 
 kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
@@ -2501,7 +2549,6 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
     return fail(KVF_ERR_INVALID_CONFIG, "misaligned rows");
   DeviceGuard g(ctx->device);
   cudaStream_t st = S(stream);
-  Scratch sc(st, ctx->pool);
   PagedAttn a;
   a.s = plan->seqs;
   a.c = paged_layer(pool, layer);
@@ -2514,95 +2561,117 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
   a.scale2 = scale * 1.44269504088896340736f;
   a.out = out;
   a.lse = lse;
+  a.part_o = plan->part_o;
+  a.part_ml = plan->part_ml;
+  a.counters = plan->counters;
   a.status = ctx->d_status;
-  if (decay >= 0.0f && !lse) {
-    a.lse = sc.get<float>(plan->tokens * plan->heads * plan->group);
-    if (!a.lse) return fail(KVF_ERR_CUDA, "scratch allocation failed");
+  KVF_TRY(plan_enter(plan, st));
+  const bool track = decay >= 0.0f;
+  if (track) {
+    if (!lse) KVF_TRY(plan_floats(plan, &plan->lse, plan->tokens * plan->heads * plan->group, st));
+    if (plan->scores_n) KVF_TRY(plan_floats(plan, &plan->scores, plan->scores_n, st));
+    if (plan->weights.parts)
+      KVF_TRY(plan_floats(plan, &plan->part_w, (size_t)2 * plan->weights.parts * kWeightSlots, st));
+    if (!lse) a.lse = plan->lse;
   }
-  float* scores = nullptr;
-  if (decay >= 0.0f && plan->decode_slots_n) {
-    scores = sc.get<float>(plan->scores_n);
-    if (!scores) return fail(KVF_ERR_CUDA, "scratch allocation failed");
-  }
-  KVF_TRY(reader_enter(plan, st));
   cudaError_t err = cudaSuccess;
   for (const PagedWork& w : plan->works) {
-    if (w.parts) {
-      const size_t rows = (size_t)w.parts * w.row_tile;
-      a.part_o = sc.get<float>(rows * plan->dim);
-      a.part_ml = sc.get<float>(rows * 2);
-      if (!a.part_o || !a.part_ml) err = cudaErrorMemoryAllocation;
+    if (err != cudaSuccess) break;
+    a.joins = w.joins;
+    if (w.kernel == kPagedDecode) {
+      err = launch_paged_decode(a, w, track ? plan->scores : nullptr, plan->score_at, st);
+    } else if (w.kernel == kPagedChunk) {
+      err = launch_paged_chunk(a, w, st);
+    } else {
+      err = launch_paged_attn_generic(a, w, st);
+      if (err == cudaSuccess) err = launch_paged_join(a, w, st);
     }
-    if (err == cudaSuccess)
-      err = w.kernel == kPagedDecode  ? launch_paged_decode(a, w, scores, plan->score_at, st)
-            : w.kernel == kPagedChunk ? launch_paged_chunk(a, w, st)
-                                      : launch_paged_attn_generic(a, w, st);
-    if (err == cudaSuccess) err = launch_paged_join(a, w, st);
   }
-  if (err == cudaSuccess && decay >= 0.0f && plan->slots_n) {
+  if (err == cudaSuccess && track && plan->slots_n) {
     err = cudaErrorNotSupported;
-    if (plan->weights.joins_n) {
-      float* part_w = sc.get<float>((size_t)2 * plan->weights.parts * kWeightSlots);
-      err = part_w ? launch_paged_chunk_weights(a, plan->weights, plan->tokens, part_w, decay, st)
-                   : cudaErrorMemoryAllocation;
-    }
+    if (plan->weights.joins_n) err = launch_paged_chunk_weights(a, plan->weights, plan->tokens, plan->part_w, decay, st);
     if (err == cudaErrorNotSupported)
       err = launch_paged_weights_generic(a, plan->slots, plan->slots_n, plan->few_rows, decay, st);
   }
-  if (err == cudaSuccess && decay >= 0.0f)
-    err = launch_paged_decode_weights(a, plan->decode_slots, plan->decode_slots_n, scores, plan->score_at, decay, st);
+  if (err == cudaSuccess && track)
+    err = launch_paged_decode_weights(a, plan->decode_slots, plan->decode_slots_n, plan->scores, plan->score_at, decay,
+                                      st);
   const kvf_status ls = reader_leave(plan, st);
   KVF_CUDA(err);
   return ls;
 }
 
-kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t budget,
-                           size_t recent, size_t sinks, const int32_t* new_table_host, size_t new_table_stride,
-                           int32_t* kept, void* stream) {
-  KVF_TRY(check_plan(ctx, plan, pool, 0));
+kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs, const int32_t* kv_lens_host,
+                           const int32_t* page_table_host, size_t table_stride, size_t budget, size_t recent,
+                           size_t sinks, const int32_t* new_table_host, size_t new_table_stride, int32_t* kept,
+                           void* stream) {
+  KVF_TRY(check_ctx(ctx));
+  KVF_TRY(check_pool(pool));
   if (!pool->weights) return fail(KVF_ERR_INVALID_CONFIG, "the pool keeps no weights");
   if (budget == 0 || budget > kMaxLen) return fail(KVF_ERR_INVALID_CONFIG, "budget must be in 1..2^30");
   if (recent > budget || sinks > budget - recent)
     return fail(KVF_ERR_INVALID_CONFIG, "sinks and recent slots exceed the budget");
-  const size_t n = plan->kv_lens.size();
+  const size_t n = num_seqs;
   if (n == 0) return KVF_OK;
-  if (!new_table_host || !kept) return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
+  if (n > 65535 || n * pool->num_heads > 65535)
+    return fail(KVF_ERR_SHAPE_MISMATCH, "num_seqs * num_heads > 65535 is not supported");
+  if (!kv_lens_host || !page_table_host || !new_table_host || !kept)
+    return fail(KVF_ERR_INVALID_CONFIG, "null pointer");
   DeviceGuard g(ctx->device);
   cudaStream_t st = S(stream);
   Scratch sc(st, ctx->pool);
-  int* table = nullptr;
-  size_t stride = 1;
   try {  // no exception leaves the C ABI
-    std::vector<bool> used(plan->num_pages, false);
-    for (const int id : plan->pages) used[id] = true;
-    std::vector<size_t> count(n);
+    std::vector<int> seen;  // source pages, then the new ones
+    size_t stride = 1, new_stride = 1, longest = 0;
+    auto pages_of = [&](size_t slots) { return (slots + pool->page_size - 1) / pool->page_size; };
     for (size_t i = 0; i < n; ++i) {
-      const size_t m = std::min(budget, (size_t)plan->kv_lens[i]);
-      count[i] = (m + plan->page_size - 1) / plan->page_size;
-      if (count[i] > new_table_stride) return fail(KVF_ERR_SHAPE_MISMATCH, "page table shorter than the budget");
-      stride = std::max(stride, count[i]);
+      if (kv_lens_host[i] < 0 || (size_t)kv_lens_host[i] > kMaxLen)
+        return fail(KVF_ERR_SHAPE_MISMATCH, "sequence lengths must be in 0..2^30");
+      longest = std::max(longest, (size_t)kv_lens_host[i]);
     }
-    std::vector<int> host(n * stride, 0);
-    for (size_t i = 0; i < n; ++i)
-      for (size_t k = 0; k < count[i]; ++k) {
-        const int32_t id = new_table_host[i * new_table_stride + k];
-        if (id < 0 || (size_t)id >= plan->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
-        if (used[id]) return fail(KVF_ERR_INVALID_CONFIG, "a new page is in use");
-        used[id] = true;
-        host[i * stride + k] = id;
+    stride = std::max(stride, pages_of(longest));
+    new_stride = std::max(new_stride, pages_of(std::min(budget, longest)));
+    std::vector<int> tables(n + n * stride + n * new_stride, 0);
+    for (size_t i = 0; i < n; ++i) {
+      const size_t len = (size_t)kv_lens_host[i];
+      tables[i] = kv_lens_host[i];
+      const size_t count = pages_of(len);
+      if (count > table_stride) return fail(KVF_ERR_SHAPE_MISMATCH, "page table shorter than a sequence");
+      for (size_t k = 0; k < count; ++k) {
+        const int32_t id = page_table_host[i * table_stride + k];
+        if (id < 0 || (size_t)id >= pool->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
+        tables[n + i * stride + k] = id;
+        seen.push_back(id);
       }
-    table = sc.get<int>(host.size());
-    if (!table) return fail(KVF_ERR_CUDA, "scratch allocation failed");
-    KVF_TRY(upload(ctx, table, host.data(), host.size() * sizeof(int), st));
+    }
+    // (sequences may share pages that are only read)
+    std::sort(seen.begin(), seen.end());
+    seen.erase(std::unique(seen.begin(), seen.end()), seen.end());
+    for (size_t i = 0; i < n; ++i) {
+      const size_t count = pages_of(std::min(budget, (size_t)kv_lens_host[i]));
+      if (count > new_table_stride) return fail(KVF_ERR_SHAPE_MISMATCH, "page table shorter than the budget");
+      for (size_t k = 0; k < count; ++k) {
+        const int32_t id = new_table_host[i * new_table_stride + k];
+        if (id < 0 || (size_t)id >= pool->num_pages) return fail(KVF_ERR_SHAPE_MISMATCH, "page outside the pool");
+        tables[n + n * stride + i * new_stride + k] = id;
+        seen.push_back(id);
+      }
+    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+      return fail(KVF_ERR_INVALID_CONFIG, "a new page is in use");
+    int* dev = nullptr;
+    if (tables.size() > (size_t)kPageListMax) {
+      dev = sc.get<int>(tables.size());
+      if (!dev) return fail(KVF_ERR_CUDA, "scratch allocation failed");
+      KVF_TRY(upload(ctx, dev, tables.data(), tables.size() * sizeof(int), st));
+    }
+    KVF_CUDA(launch_paged_evict(tables.data(), dev, n, stride, new_stride, longest, paged_layer(pool, 0),
+                                pool->num_layers, budget, recent, sinks, kept, st));
   } catch (const std::exception& ex) {
     return fail(KVF_ERR_PIPELINE, std::string("paged eviction: ") + ex.what());
   }
-  KVF_TRY(reader_enter(plan, st));
-  const cudaError_t err = launch_paged_evict(plan->seqs, paged_layer(pool, 0), pool->num_layers, budget, recent, sinks,
-                                             table, stride, kept, st);
-  const kvf_status ls = reader_leave(plan, st);
-  KVF_CUDA(err);
-  return ls;
+  return KVF_OK;
 }
 
 }  // extern "C"

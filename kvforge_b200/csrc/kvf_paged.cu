@@ -50,15 +50,19 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
             if (!fresh && left - fixed < std::min(least, count - it)) close();
             int take = (int)std::min<long long>(count - it, std::max<long long>(left - fixed, 1));
             if (count - it - take < least) take = count - it;  // no sliver behind the cut
-            out->segs.push_back({(int)i, h, r, it, it + take, -1});
+            out->segs.push_back({(int)i, h, r, it, it + take, -1, -1});
             it += take;
             left -= take + fixed;
             if (left <= fixed) close();
           } while (it < count);
           const int parts = (int)(out->segs.size() - seg0);
           if (parts > 1) {
+            for (size_t k = seg0; k < out->segs.size(); ++k) {
+              out->segs[k].part = out->parts + (int)(k - seg0);
+              out->segs[k].join = (int)out->joins.size();
+            }
             out->joins.push_back({(int)i, h, r, out->parts, parts});
-            for (size_t k = seg0; k < out->segs.size(); ++k) out->segs[k].part = out->parts++;
+            out->parts += parts;
           }
         }
     }
@@ -73,78 +77,77 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
 namespace {
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyUnroll = 4;
+constexpr int kRowsPerWarp = 8;
 
-// sequence of token t: the last i with q_start[i] <= t
-__device__ __forceinline__ int seq_of(const PagedSeqs& s, int t) {
-  int lo = 0, hi = s.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(s.q_start + mid) <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
-// New rows into pages. A unit is one V (16 bytes, or one element where rows
-// are not 16-byte aligned) of the key or value of one (token, head); every
-// thread has kCopyUnroll units in flight. Bound by HBM (each byte read once
-// and written once).
+// New rows into pages. A warp takes kRowsPerWarp (token, head) pairs, whose
+// places lanes 0-7 look up, and has all their loads in flight before the first
+// store; a unit is one V (16 bytes, or one element where rows are not 16-byte
+// aligned). `place` holds every token's page and row (page * 128 + row, -1
+// where a query lies in front of slot 0). Bound by HBM: each byte is read once
+// and written once.
 template <typename V>
-__global__ void __launch_bounds__(kCopyThreads) k_paged_append(PagedSeqs s, PagedLayer c, unsigned units,
-                                                               unsigned row_units, const V* __restrict__ k, size_t kt,
+__global__ void __launch_bounds__(kCopyThreads) k_paged_append(const long long* __restrict__ place, PagedLayer c,
+                                                               unsigned units, const V* __restrict__ k, size_t kt,
                                                                size_t kh, const V* __restrict__ v, size_t vt,
-                                                               size_t vh, size_t tokens) {
-  const unsigned per_token = units;  // heads * 2 * row_units
-  const size_t total = tokens * per_token;
-  const size_t base = (size_t)blockIdx.x * (kCopyThreads * kCopyUnroll) + threadIdx.x;
-  V x[kCopyUnroll];
-  V* dst[kCopyUnroll];
-#pragma unroll
-  for (int u = 0; u < kCopyUnroll; ++u) {
-    const size_t i = base + (size_t)u * kCopyThreads;
-    dst[u] = nullptr;
-    if (i >= total) continue;
-    const size_t t = i / per_token;
-    unsigned r = (unsigned)(i - t * per_token);
-    const unsigned which = r / (units >> 1);
-    r -= which * (units >> 1);
-    const unsigned h = r / row_units, e = r - h * row_units;
-    const int b = seq_of(s, (int)t);
-    const int q1 = __ldg(s.q_start + b + 1);
-    const int j = __ldg(s.kv_len + b) - (q1 - (int)t);
-    if (j < 0) continue;  // a query in front of slot 0 has no slot
-    const int page = __ldg(s.table + (size_t)b * s.stride + (j >> c.page_shift));
-    const size_t row = (((size_t)page * c.heads + h) << c.page_shift) + (j & ((1 << c.page_shift) - 1));
-    x[u] = which ? v[t * vt + h * vh + e] : k[t * kt + h * kh + e];
-    dst[u] = static_cast<V*>(which ? c.values : c.keys) + row * row_units + e;
-    if (!which && e == 0 && c.weights) c.weights[row] = 0.0f;
+                                                               size_t vh, unsigned pairs) {
+  const int lane = threadIdx.x & 31;
+  const unsigned p0 = (blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kRowsPerWarp;
+  unsigned long long row = ~0ull, from_k = 0, from_v = 0;
+  if (lane < kRowsPerWarp && p0 + lane < pairs) {
+    const unsigned t = (p0 + lane) / c.heads, h = (p0 + lane) - t * c.heads;
+    const long long at = __ldg(place + t);
+    if (at >= 0) {
+      row = ((((unsigned long long)(at >> 7)) * c.heads + h) << c.page_shift) + (unsigned)(at & 127);
+      if (c.weights) c.weights[row] = 0.0f;
+    }
+    from_k = t * kt + h * kh;
+    from_v = t * vt + h * vh;
   }
+  for (unsigned e0 = 0; e0 < 2 * units; e0 += 32) {
+    const unsigned e = e0 + lane;
+    const bool val = e >= units;
+    const unsigned col = val ? e - units : e;
+    V x[kRowsPerWarp];
+    unsigned long long dst[kRowsPerWarp];
 #pragma unroll
-  for (int u = 0; u < kCopyUnroll; ++u)
-    if (dst[u]) *dst[u] = x[u];
+    for (int u = 0; u < kRowsPerWarp; ++u) {
+      dst[u] = __shfl_sync(0xffffffffu, row, u);
+      const unsigned long long sk = __shfl_sync(0xffffffffu, from_k, u), sv = __shfl_sync(0xffffffffu, from_v, u);
+      if (dst[u] != ~0ull && e < 2 * units) x[u] = val ? v[sv + col] : k[sk + col];
+    }
+    V* pool = static_cast<V*>(val ? c.values : c.keys);
+#pragma unroll
+    for (int u = 0; u < kRowsPerWarp; ++u)
+      if (dst[u] != ~0ull && e < 2 * units) pool[dst[u] * units + col] = x[u];
+  }
 }
+
+// pages of a sequence, as a kernel parameter
+struct PageList {
+  int v[kPageListMax];
+};
 
 // One (page, head) block of a sequence is contiguous on both sides: keys
-// (blockIdx.z = 0) or values, whole blocks of the page's used rows.
+// (blockIdx.z = 0) or values, whole blocks of the page's used rows. Bound by HBM.
+constexpr int kGatherUnroll = 4;
 template <typename V>
-__global__ void __launch_bounds__(kCopyThreads) k_paged_gather(const int* __restrict__ table, PagedLayer c, int len,
-                                                               unsigned row_units, V* __restrict__ k,
-                                                               V* __restrict__ v) {
-  const int j0 = (int)blockIdx.x << c.page_shift, h = blockIdx.y;
+__global__ void __launch_bounds__(kCopyThreads) k_paged_gather(const __grid_constant__ PageList pages, PagedLayer c,
+                                                               int first, int len, unsigned row_units,
+                                                               V* __restrict__ k, V* __restrict__ v) {
+  const int j0 = (first + (int)blockIdx.x) << c.page_shift, h = blockIdx.y;
   const int rows = min(1 << c.page_shift, len - j0);
-  const int page = __ldg(table + blockIdx.x);
+  const int page = pages.v[blockIdx.x];
   const V* src = static_cast<const V*>(blockIdx.z ? c.values : c.keys) +
                  (((size_t)page * c.heads + h) << c.page_shift) * row_units;
   V* dst = (blockIdx.z ? v : k) + ((size_t)h * len + j0) * row_units;
   const unsigned n = rows * row_units;
-  for (unsigned i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kCopyUnroll) {
-    V x[kCopyUnroll];
+  for (unsigned i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kGatherUnroll) {
+    V x[kGatherUnroll];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
+    for (int u = 0; u < kGatherUnroll; ++u)
       if (i0 + u * kCopyThreads < n) x[u] = __ldg(src + i0 + u * kCopyThreads);
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
+    for (int u = 0; u < kGatherUnroll; ++u)
       if (i0 + u * kCopyThreads < n) dst[i0 + u * kCopyThreads] = x[u];
   }
 }
@@ -185,18 +188,37 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
   return x - v + (w ? warp_sums[w - 1] : 0);
 }
 
+// what an eviction reads of its sequences: lengths [n], pages [n, stride], new
+// pages [n, new_stride], one behind the other; in the parameter where they fit
+struct EvictTables {
+  const int* p;  // device, or nullptr: v
+  int n, stride, new_stride;
+  int v[kPageListMax];
+  __device__ __forceinline__ const int* lens() const { return p ? p : v; }
+  __device__ __forceinline__ const int* pages(int b) const { return lens() + n + (size_t)b * stride; }
+  __device__ __forceinline__ const int* new_pages(int b) const {
+    return lens() + n + (size_t)n * stride + (size_t)b * new_stride;
+  }
+};
+
 // Which slots stay, one CTA per (head, sequence, layer). The threshold among
 // the slots that compete (all but the sinks and the recent ones) is the
 // need-th largest key, found by a radix selection over three histograms of
-// the key's bits; then one pass in slot order writes the kept slots: those
-// above the threshold, and the first `ties` of those equal to it. Integer
+// the key's bits; then every thread takes a run of slots and, after prefix sums
+// over the runs' counts, writes those of its run that stay, in order: those
+// above the threshold, and the first `need` of those equal to it. The keys are
+// kept in shared memory (one word of padding after 32, so that runs start in
+// different banks) where they fit, and read again from L2 otherwise. Integer
 // counts only, so the result does not depend on the order of the atomics.
-__global__ void __launch_bounds__(kSelThreads) k_paged_select(PagedSeqs s, PagedLayer c, int budget, int recent,
-                                                              int sinks, int* __restrict__ kept) {
+// Bound by latencies: four passes of a CTA over its keys.
+__global__ void __launch_bounds__(kSelThreads) k_paged_select(const __grid_constant__ EvictTables tab, PagedLayer c,
+                                                              int budget, int recent, int sinks, int cached,
+                                                              int* __restrict__ kept) {
+  extern __shared__ uint32_t keys[];  // [cached + cached / 32 + 1]
   const int h = blockIdx.x, b = blockIdx.y;
   const size_t layer = blockIdx.z;
-  const int n = __ldg(s.kv_len + b);
-  int* out = kept + ((layer * s.n + b) * c.heads + h) * (size_t)budget;
+  const int n = tab.lens()[b];
+  int* out = kept + ((layer * tab.n + b) * c.heads + h) * (size_t)budget;
   const int tid = threadIdx.x;
   if (n <= budget) {
     for (int i = tid; i < budget; i += kSelThreads) out[i] = i < n ? i : -1;
@@ -206,23 +228,31 @@ __global__ void __launch_bounds__(kSelThreads) k_paged_select(PagedSeqs s, Paged
   __shared__ int warp_sums[32];
   __shared__ uint32_t sh_prefix;
   __shared__ int sh_need;
-  const int* table = s.table + (size_t)b * s.stride;
+  const int* table = tab.pages(b);
   const int mask = (1 << c.page_shift) - 1;
   const float* w = c.weights + (((layer * c.pages) * c.heads) << c.page_shift);
-  auto key_at = [&](int j) {
-    const int page = __ldg(table + (j >> c.page_shift));
-    return weight_key(__ldg(w + (((size_t)page * c.heads + h) << c.page_shift) + (j & mask)));
+  auto load_key = [&](int j) {
+    return weight_key(w[(((size_t)table[j >> c.page_shift] * c.heads + h) << c.page_shift) + (j & mask)]);
   };
+  const bool have = n <= cached;
+  if (have) {
+#pragma unroll 8
+    for (int j = tid; j < n; j += kSelThreads) keys[j + (j >> 5)] = load_key(j);
+    __syncthreads();
+  }
+  auto key_at = [&](int j) { return have ? keys[j + (j >> 5)] : load_key(j); };
   const int j0 = sinks, j1 = n - recent;  // sinks + recent <= budget < n
   int need = budget - sinks - recent;
+  const bool any = need > 0;
   uint32_t prefix = 0, known = 0;  // the threshold's leading bits, and which they are
-  if (need > 0) {
+  if (any) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int bits = pass == 2 ? 32 - 2 * kSelBits : kSelBits;
       const int shift = pass == 0 ? 32 - kSelBits : pass == 1 ? 32 - 2 * kSelBits : 0;
       for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
+#pragma unroll 4
       for (int j = j0 + tid; j < j1; j += kSelThreads) {
         const uint32_t u = key_at(j);
         if ((u & known) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1);
@@ -246,144 +276,155 @@ __global__ void __launch_bounds__(kSelThreads) k_paged_select(PagedSeqs s, Paged
     }
   }
   // need: how many of the slots equal to the threshold stay, the lowest first
-  const bool any = budget - sinks - recent > 0;
-  int at = 0, ties = 0;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int j = base + tid;
-    bool keep = false, tie = false;
-    if (j < n) {
-      if (j < j0 || j >= j1) keep = true;
-      else if (any) {
-        const uint32_t u = key_at(j);
-        keep = u > prefix;
-        tie = u == prefix;
-      }
+  const int run = (n + kSelThreads - 1) / kSelThreads;
+  const int i0 = min(n, tid * run), i1 = min(n, i0 + run);
+  int keep = 0, ties = 0;
+  for (int j = i0; j < i1; ++j) {
+    if (j < j0 || j >= j1) {
+      ++keep;
+    } else if (any) {
+      const uint32_t u = key_at(j);
+      keep += u > prefix;
+      ties += u == prefix;
     }
-    int sum;
-    // both counts in one scan: at most 1024 of each
-    const int pre = block_scan((keep ? 1 : 0) | (tie ? 1 << 16 : 0), warp_sums, &sum);
-    const int tie_pre = ties + (pre >> 16);
-    if (tie && tie_pre < need) keep = true;
-    // of the ties in front of this slot, the first `need` of all are kept
-    const int pos = at + (pre & 0xffff) + min(max(need - ties, 0), pre >> 16);
-    if (keep) out[pos] = j;
-    at += (sum & 0xffff) + min(max(need - ties, 0), sum >> 16);
-    ties += sum >> 16;
+  }
+  int total;
+  const int keep0 = block_scan(keep, warp_sums, &total), ties0 = block_scan(ties, warp_sums, &total);
+  int pos = keep0 + (any ? min(ties0, need) : 0), left = any ? max(0, need - ties0) : 0;
+  for (int j = i0; j < i1; ++j) {
+    bool stays = j < j0 || j >= j1;
+    if (!stays && any) {
+      const uint32_t u = key_at(j);
+      stays = u > prefix || (u == prefix && left-- > 0);
+    }
+    if (stays) out[pos++] = j;
   }
 }
 
-// Kept rows into their new pages. A unit is one V of the key or value of one
-// kept slot; bound by HBM.
+// Kept rows into their new pages, kRowsPerWarp slots per warp; bound by HBM.
 template <typename V>
-__global__ void __launch_bounds__(kCopyThreads) k_paged_move(PagedSeqs s, PagedLayer c, int budget,
-                                                             const int* __restrict__ new_table, size_t new_stride,
-                                                             const int* __restrict__ kept, unsigned row_units) {
+__global__ void __launch_bounds__(kCopyThreads) k_paged_move(const __grid_constant__ EvictTables tab, PagedLayer c,
+                                                             int budget, const int* __restrict__ kept,
+                                                             unsigned units) {
   const int bh = blockIdx.y, h = bh % c.heads, b = bh / c.heads;
   const size_t layer = blockIdx.z;
-  const int m = min(__ldg(s.kv_len + b), budget);
-  const int* from = kept + ((layer * s.n + b) * c.heads + h) * (size_t)budget;
-  const int* table = s.table + (size_t)b * s.stride;
-  const int* to = new_table + (size_t)b * new_stride;
-  const size_t layer_rows = ((size_t)c.pages * c.heads) << c.page_shift;
+  const int m = min(tab.lens()[b], budget), lane = threadIdx.x & 31;
+  const int r0 = (blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kRowsPerWarp;
+  if (r0 >= m) return;
   const int mask = (1 << c.page_shift) - 1;
-  const size_t total = (size_t)m * 2 * row_units;
-  const size_t base = (size_t)blockIdx.x * (kCopyThreads * kCopyUnroll) + threadIdx.x;
-  V x[kCopyUnroll];
-  V* dst[kCopyUnroll];
-#pragma unroll
-  for (int u = 0; u < kCopyUnroll; ++u) {
-    const size_t i = base + (size_t)u * kCopyThreads;
-    dst[u] = nullptr;
-    if (i >= total) continue;
-    const unsigned r = (unsigned)(i / (2 * row_units)), f = (unsigned)(i - (size_t)r * (2 * row_units));
-    const bool val = f >= row_units;
-    const unsigned e = val ? f - row_units : f;
-    const int j = __ldg(from + r);
-    const size_t src = layer * layer_rows +
-                       (((size_t)__ldg(table + (j >> c.page_shift)) * c.heads + h) << c.page_shift) + (j & mask);
-    const size_t row =
-        layer * layer_rows + (((size_t)__ldg(to + (r >> c.page_shift)) * c.heads + h) << c.page_shift) + (r & mask);
-    V* pool = static_cast<V*>(val ? c.values : c.keys);
-    x[u] = pool[src * row_units + e];
-    dst[u] = pool + row * row_units + e;
-    if (f == 0) c.weights[row] = c.weights[src];
+  const unsigned long long rows = layer * (((unsigned long long)c.pages * c.heads) << c.page_shift);
+  unsigned long long from = ~0ull, to = 0;
+  if (lane < kRowsPerWarp && r0 + lane < m) {
+    const int r = r0 + lane;
+    const int j = __ldg(kept + ((layer * tab.n + b) * c.heads + h) * (size_t)budget + r);
+    from = rows + (((unsigned long long)tab.pages(b)[j >> c.page_shift] * c.heads + h) << c.page_shift) + (j & mask);
+    to = rows + (((unsigned long long)tab.new_pages(b)[r >> c.page_shift] * c.heads + h) << c.page_shift) + (r & mask);
+    c.weights[to] = c.weights[from];
   }
+  for (unsigned e0 = 0; e0 < 2 * units; e0 += 32) {
+    const unsigned e = e0 + lane;
+    const bool val = e >= units;
+    const unsigned col = val ? e - units : e;
+    V* pool = static_cast<V*>(val ? c.values : c.keys);
+    V x[kRowsPerWarp];
 #pragma unroll
-  for (int u = 0; u < kCopyUnroll; ++u)
-    if (dst[u]) *dst[u] = x[u];
+    for (int u = 0; u < kRowsPerWarp; ++u) {
+      const unsigned long long src = __shfl_sync(0xffffffffu, from, u);
+      if (src != ~0ull && e < 2 * units) x[u] = __ldcs(pool + src * units + col);
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsPerWarp; ++u) {
+      const unsigned long long src = __shfl_sync(0xffffffffu, from, u), dst = __shfl_sync(0xffffffffu, to, u);
+      if (src != ~0ull && e < 2 * units) pool[dst * units + col] = x[u];
+    }
+  }
 }
 
 size_t elem_size(int dtype) { return dtype == KVF_IN_F32 ? 4 : 2; }
 
 template <typename V>
-cudaError_t append_typed(const PagedSeqs& s, const PagedLayer& c, size_t tokens, const void* k, size_t kt, size_t kh,
-                         const void* v, size_t vt, size_t vh, cudaStream_t st) {
+cudaError_t append_typed(const long long* place, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
+                         size_t kh, const void* v, size_t vt, size_t vh, cudaStream_t st) {
   const size_t e = elem_size(c.dtype), per = sizeof(V) / e;
-  const unsigned row_units = (unsigned)(c.dim / per), units = (unsigned)(2 * row_units * c.heads);
-  const size_t blocks = (tokens * units + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll);
-  if (blocks > 0x7fffffffu) return cudaErrorInvalidValue;
-  k_paged_append<V><<<(unsigned)blocks, kCopyThreads, 0, st>>>(s, c, units, row_units, static_cast<const V*>(k),
-                                                               kt / per, kh / per, static_cast<const V*>(v), vt / per,
-                                                               vh / per, tokens);
+  const size_t pairs = tokens * c.heads, per_block = kCopyThreads / 32 * kRowsPerWarp;
+  if (pairs > 0x7fffffffu) return cudaErrorInvalidValue;
+  k_paged_append<V><<<(unsigned)((pairs + per_block - 1) / per_block), kCopyThreads, 0, st>>>(
+      place, c, (unsigned)(c.dim / per), static_cast<const V*>(k), kt / per, kh / per, static_cast<const V*>(v),
+      vt / per, vh / per, (unsigned)pairs);
   note_launches(1);
   return cudaGetLastError();
 }
 
 template <typename V>
-cudaError_t gather_typed(const PagedSeqs& s, const PagedLayer& c, size_t seq, size_t len, void* k, void* v,
-                         cudaStream_t st) {
+cudaError_t gather_typed(const int* pages, const PagedLayer& c, size_t len, void* k, void* v, cudaStream_t st) {
   const unsigned row_units = (unsigned)(c.dim * elem_size(c.dtype) / sizeof(V));
-  const size_t page = (size_t)1 << c.page_shift;
-  const dim3 grid((unsigned)((len + page - 1) / page), (unsigned)c.heads, 2);
-  k_paged_gather<V><<<grid, kCopyThreads, 0, st>>>(s.table + seq * s.stride, c, (int)len, row_units,
-                                                   static_cast<V*>(k), static_cast<V*>(v));
-  note_launches(1);
+  const size_t page = (size_t)1 << c.page_shift, n = (len + page - 1) / page;
+  for (size_t first = 0; first < n; first += kPageListMax) {
+    const size_t m = std::min<size_t>(kPageListMax, n - first);
+    PageList list;
+    std::copy(pages + first, pages + first + m, list.v);
+    k_paged_gather<V><<<dim3((unsigned)m, (unsigned)c.heads, 2), kCopyThreads, 0, st>>>(
+        list, c, (int)first, (int)len, row_units, static_cast<V*>(k), static_cast<V*>(v));
+    note_launches(1);
+  }
   return cudaGetLastError();
 }
 
 template <typename V>
-cudaError_t move_typed(const PagedSeqs& s, const PagedLayer& c, size_t layers, size_t budget, const int* new_table,
-                       size_t new_stride, const int* kept, cudaStream_t st) {
-  const unsigned row_units = (unsigned)(c.dim * elem_size(c.dtype) / sizeof(V));
-  const size_t per = kCopyThreads * kCopyUnroll;
-  const size_t blocks = (budget * 2 * row_units + per - 1) / per;
-  if (blocks > 0x7fffffffu) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)blocks, (unsigned)(s.n * c.heads), (unsigned)layers);
-  k_paged_move<V><<<grid, kCopyThreads, 0, st>>>(s, c, (int)budget, new_table, new_stride, kept, row_units);
+cudaError_t move_typed(const EvictTables& tab, const PagedLayer& c, size_t layers, size_t budget, const int* kept,
+                       cudaStream_t st) {
+  const unsigned units = (unsigned)(c.dim * elem_size(c.dtype) / sizeof(V));
+  const size_t per = kCopyThreads / 32 * kRowsPerWarp;
+  const dim3 grid((unsigned)((budget + per - 1) / per), (unsigned)(tab.n * c.heads), (unsigned)layers);
+  k_paged_move<V><<<grid, kCopyThreads, 0, st>>>(tab, c, (int)budget, kept, units);
   note_launches(1);
   return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_paged_append(const PagedSeqs& s, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
+cudaError_t launch_paged_append(const long long* place, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
                                 size_t kh, const void* v, size_t vt, size_t vh, cudaStream_t st) {
   const size_t e = elem_size(c.dtype);
   const bool wide = c.dim * e % 16 == 0 && (kt | kh | vt | vh) * e % 16 == 0 && aligned(k, 16) && aligned(v, 16);
-  if (wide) return append_typed<uint4>(s, c, tokens, k, kt, kh, v, vt, vh, st);
-  if (e == 4) return append_typed<uint32_t>(s, c, tokens, k, kt, kh, v, vt, vh, st);
-  return append_typed<uint16_t>(s, c, tokens, k, kt, kh, v, vt, vh, st);
+  if (wide) return append_typed<uint4>(place, c, tokens, k, kt, kh, v, vt, vh, st);
+  if (e == 4) return append_typed<uint32_t>(place, c, tokens, k, kt, kh, v, vt, vh, st);
+  return append_typed<uint16_t>(place, c, tokens, k, kt, kh, v, vt, vh, st);
 }
 
-cudaError_t launch_paged_gather(const PagedSeqs& s, const PagedLayer& c, size_t seq, size_t len, void* k, void* v,
+cudaError_t launch_paged_gather(const int* pages, const PagedLayer& c, size_t len, void* k, void* v,
                                 cudaStream_t st) {
   const size_t e = elem_size(c.dtype);
-  if (c.dim * e % 16 == 0 && aligned(k, 16) && aligned(v, 16)) return gather_typed<uint4>(s, c, seq, len, k, v, st);
-  if (e == 4) return gather_typed<uint32_t>(s, c, seq, len, k, v, st);
-  return gather_typed<uint16_t>(s, c, seq, len, k, v, st);
+  if (c.dim * e % 16 == 0 && aligned(k, 16) && aligned(v, 16)) return gather_typed<uint4>(pages, c, len, k, v, st);
+  if (e == 4) return gather_typed<uint32_t>(pages, c, len, k, v, st);
+  return gather_typed<uint16_t>(pages, c, len, k, v, st);
 }
 
-cudaError_t launch_paged_evict(const PagedSeqs& s, const PagedLayer& c, size_t layers, size_t budget, size_t recent,
-                               size_t sinks, const int* new_table, size_t new_stride, int* kept, cudaStream_t st) {
-  const dim3 grid((unsigned)c.heads, (unsigned)s.n, (unsigned)layers);
-  k_paged_select<<<grid, kSelThreads, 0, st>>>(s, c, (int)budget, (int)recent, (int)sinks, kept);
+cudaError_t launch_paged_evict(const int* tables, const int* tables_dev, size_t n, size_t stride, size_t new_stride,
+                               size_t longest, const PagedLayer& c, size_t layers, size_t budget, size_t recent,
+                               size_t sinks, int* kept, cudaStream_t st) {
+  EvictTables tab;
+  tab.p = tables_dev;
+  tab.n = (int)n;
+  tab.stride = (int)stride;
+  tab.new_stride = (int)new_stride;
+  if (!tables_dev) std::copy(tables, tables + n + n * stride + n * new_stride, tab.v);
+  // as many keys as shared memory holds
+  constexpr size_t kKeyMost = 50 * 1024;
+  const size_t cached = std::min(longest, kKeyMost), smem = (cached + cached / 32 + 1) * 4;
+  cudaError_t e = cudaSuccess;
+  if (smem > kSmemOptIn - sizeof(int) * kSelBins)
+    e = cudaFuncSetAttribute(k_paged_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)c.heads, (unsigned)n, (unsigned)layers);
+  k_paged_select<<<grid, kSelThreads, smem, st>>>(tab, c, (int)budget, (int)recent, (int)sinks, (int)cached, kept);
   note_launches(1);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const size_t es = elem_size(c.dtype);
-  if (c.dim * es % 16 == 0) return move_typed<uint4>(s, c, layers, budget, new_table, new_stride, kept, st);
-  if (es == 4) return move_typed<uint32_t>(s, c, layers, budget, new_table, new_stride, kept, st);
-  return move_typed<uint16_t>(s, c, layers, budget, new_table, new_stride, kept, st);
+  if (c.dim * es % 16 == 0) return move_typed<uint4>(tab, c, layers, budget, kept, st);
+  if (es == 4) return move_typed<uint32_t>(tab, c, layers, budget, kept, st);
+  return move_typed<uint16_t>(tab, c, layers, budget, kept, st);
 }
 
 }  // namespace kvf

@@ -33,9 +33,10 @@ struct PagedSeqs {
 // and an iteration is one tile of `key_tile` slots. One CTA walks the segments
 // [first[cta], first[cta + 1]), each a range of iterations of one row tile. A
 // tile cut into several segments leaves partial results (part >= 0: their
-// slot) that are joined afterwards; part = -1 writes the output itself.
+// slot) that are joined (join: the tile's PagedJoin) by whichever writes the
+// last of them, or afterwards; part = -1 writes the output itself.
 struct PagedSeg {
-  int seq, head, row0, it0, it1, part;
+  int seq, head, row0, it0, it1, part, join;
 };
 struct PagedJoin {
   int seq, head, row0, part0, parts;
@@ -97,8 +98,11 @@ struct PagedAttn {
   float* lse = nullptr;            // [tokens, heads * group] or nullptr
   float* part_o = nullptr;         // [parts, row_tile, dim] sums before the division
   float* part_ml = nullptr;        // [parts, row_tile, 2] maximum (base 2) and sum
+  const PagedJoin* joins = nullptr;
+  unsigned* counters = nullptr;  // [joins, kJoinCounters] of arrived parts, zero between launches
   unsigned* status = nullptr;
 };
+constexpr int kJoinCounters = 8;
 
 // host side of a work list
 struct PagedWorkHost {
@@ -117,18 +121,25 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
                  PagedWorkHost* out);
 
 // ---- launchers ---------------------------------------------------------------
-cudaError_t launch_paged_append(const PagedSeqs& s, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
+// place [tokens]: page * 128 + row of every token, -1 for none
+cudaError_t launch_paged_append(const long long* place, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
                                 size_t kh, const void* v, size_t vt, size_t vh, cudaStream_t st);
-cudaError_t launch_paged_gather(const PagedSeqs& s, const PagedLayer& c, size_t seq, size_t len, void* k, void* v,
-                                cudaStream_t st);
-// layers stacked `pages` apart; kept [layers, n, heads, budget]
-cudaError_t launch_paged_evict(const PagedSeqs& s, const PagedLayer& c, size_t layers, size_t budget, size_t recent,
-                               size_t sinks, const int* new_table, size_t new_stride, int* kept, cudaStream_t st);
+// host arrays of pages up to this many words travel as kernel parameters
+constexpr int kPageListMax = 960;
+// pages: the sequence's, on the host
+cudaError_t launch_paged_gather(const int* pages, const PagedLayer& c, size_t len, void* k, void* v, cudaStream_t st);
+// tables (host): lengths [n], pages [n, stride], new pages [n, new_stride], one
+// behind the other, and the same on the device, or nullptr when they are at most
+// kPageListMax words; longest: the largest length; layers stacked `pages` apart;
+// kept [layers, n, heads, budget]
+cudaError_t launch_paged_evict(const int* tables, const int* tables_dev, size_t n, size_t stride, size_t new_stride,
+                               size_t longest, const PagedLayer& c, size_t layers, size_t budget, size_t recent,
+                               size_t sinks, int* kept, cudaStream_t st);
 
 // CUDA-core attention: every type and head_dim up to 256
 constexpr int kGenRows = 64, kGenRowsShort = 16, kGenKeys = 64;
 cudaError_t launch_paged_attn_generic(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
-// joins the partial results of cut tiles
+// joins the partial results of its cut tiles
 cudaError_t launch_paged_join(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
 // weight = decay * weight + column sums of the softmax, from a.lse (natural
 // logarithm): CUDA cores, every type; slots: tiles of kGenKeys slots

@@ -77,7 +77,7 @@ void paged_split_slots(const int* q_lens, const int* kv_lens, size_t n, int head
             if (left - kFixed < std::min(4, t1 - t0) && left < quota) close();
             int take = (int)std::min<long long>(t1 - t0, std::max<long long>(left - kFixed, 1));
             if (t1 - t0 - take < 4) take = t1 - t0;
-            out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++});
+            out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++, -1});
             t0 += take;
             left -= take + kFixed;
             if (left <= kFixed) close();

@@ -10,6 +10,7 @@ include/kvforge.h); this module keeps the page tables.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 from typing import List, NamedTuple, Optional, Sequence
@@ -20,7 +21,23 @@ import torch
 from . import _lib as L
 from ._lib import KvForgeError
 
+# the current stream's handle without making a Stream object (1.2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
 _DTYPES = {torch.float32: L.IN_F32, torch.float16: L.IN_F16, torch.bfloat16: L.IN_BF16}
+
+
+def _ints(rows):
+    """Lists of whole numbers as one host array of 32-bit rows of equal length
+    (filled up with 0), and that length."""
+    n = max([1] + [len(r) for r in rows])
+    a = array.array("i", [0]) if not rows else array.array("i")
+    for r in rows:
+        a.extend(r)
+        if len(r) < n:
+            a.frombytes(bytes(4 * (n - len(r))))
+    return (C.c_int32 * len(a)).from_buffer(a), n
 
 
 class Eviction(NamedTuple):
@@ -96,10 +113,12 @@ class PagedKVCache:
                                  self.weights.data_ptr())
         self._pool_ref = C.byref(self._pool)
         self._lib, self._ctx = L.lib(), L.context(self._dev)
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         self._free = list(range(self.num_pages - 1, -1, -1))  # the lowest page is handed out first
         self._seqs = {}
         self._next = 0
         self._last = torch.cuda.current_stream(self._dev)
+        self._last_raw = self._last.cuda_stream
 
     # ---- sequences ------------------------------------------------------------
     @property
@@ -212,31 +231,25 @@ class PagedKVCache:
         np.cumsum(q, out=starts[1:])
         return PagedBatch(h, seqs, states, int(query_heads), starts)
 
-    def _table(self, lists) -> np.ndarray:
-        table = np.zeros((max(1, len(lists)), max([1] + [len(p) for p in lists])), np.int32)
-        for row, p in zip(table, lists):
-            row[:len(p)] = p
-        return table
-
     def _plan(self, states, q, query_heads, window, sinks) -> C.c_void_p:
-        table = self._table([s.pages for s in states])
-        kv = np.array([s.length for s in states], np.int32)
-        ql = np.array(q, np.int32)
+        kv, _ = _ints([[s.length for s in states]])
+        ql, _ = _ints([q])
+        table, stride = _ints([s.pages for s in states])
         h = C.c_void_p()
-        L.check(self._lib.kvf_paged_plan_create(
-            self._ctx, self._pool_ref, len(states), ql.ctypes.data, kv.ctypes.data, table.ctypes.data,
-            table.shape[1], int(query_heads), int(window), int(sinks), C.byref(h), self._enter()))
+        L.check(self._lib.kvf_paged_plan_create(self._ctx, self._pool_ref, len(states), ql, kv, table, stride,
+                                                int(query_heads), int(window), int(sinks), C.byref(h), self._enter()))
         return h
 
     def _enter(self) -> int:
         """The current stream, ordered behind the last call's."""
-        s = torch.cuda.current_stream(self._dev)
-        if s != self._last:
+        raw = _raw_stream(self._dev)
+        if raw != self._last_raw:
+            s = torch.cuda.current_stream(self._dev)
             s.wait_stream(self._last)
             for t in (self.keys, self.values, self.weights):
                 t.record_stream(s)  # the pool's memory is not reused before this stream is done with it
-            self._last = s
-        return s.cuda_stream
+            self._last, self._last_raw = s, raw
+        return raw
 
     def _handle(self, batch: PagedBatch):
         for s in batch._states:
@@ -286,11 +299,11 @@ class PagedKVCache:
         q = self._rows(query, "query", batch.tokens, batch.query_heads)
         if decay is not None and not 0.0 <= decay <= 1.0:
             raise KvForgeError(L.ERR_INVALID_CONFIG, "decay must be in 0..1")
-        out = torch.empty(q.shape, dtype=self.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = self.weights.new_empty(q.shape[:2]) if return_lse else None
         L.check(self._lib.kvf_paged_attention(
             self._ctx, h, self._pool_ref, self._layer(layer), q.data_ptr(), q.stride(0), q.stride(1),
-            1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), -1.0 if decay is None else float(decay),
+            self._scale if scale is None else float(scale), -1.0 if decay is None else float(decay),
             out.data_ptr(), lse.data_ptr() if return_lse else None, self._enter()))
         return (out, lse) if return_lse else out
 
@@ -307,24 +320,23 @@ class PagedKVCache:
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
             raise KvForgeError(L.ERR_INVALID_CONFIG, "budget must be at least 1 and hold the sinks and recent tokens")
         states = [self._seqs[s] for s in seqs]
-        h = self._plan(states, [0] * len(states), 0, 0, 0)
+        lens = [min(budget, s.length) for s in states]
+        taken = self._take(sum(self._pages_for(n) for n in lens))
+        lists, at = [], 0
+        for n in lens:
+            lists.append(taken[at:at + self._pages_for(n)])
+            at += len(lists[-1])
+        kept = self.weights.new_empty((self.num_layers, len(seqs), self.num_heads, budget), dtype=torch.int32)
         try:
-            lens = [min(budget, s.length) for s in states]
-            new = [self._pages_for(n) for n in lens]
-            taken = self._take(sum(new))
-            at = np.concatenate([[0], np.cumsum(new)]).astype(int)
-            lists = [taken[at[i]:at[i + 1]] for i in range(len(new))]
-            table = self._table(lists)
-            kept = torch.empty((self.num_layers, len(seqs), self.num_heads, budget), dtype=torch.int32,
-                               device=self.keys.device)
-            try:
-                L.check(self._lib.kvf_paged_evict(self._ctx, h, self._pool_ref, budget, int(recent), int(sinks),
-                                                  table.ctypes.data, table.shape[1], kept.data_ptr(), self._enter()))
-            except Exception:
-                self._give(taken)
-                raise
-        finally:
-            self._lib.kvf_paged_plan_free(h)
+            kv, _ = _ints([[s.length for s in states]])
+            table, stride = _ints([s.pages for s in states])
+            new, new_stride = _ints(lists)
+            L.check(self._lib.kvf_paged_evict(self._ctx, self._pool_ref, len(states), kv, table, stride, budget,
+                                              int(recent), int(sinks), new, new_stride, kept.data_ptr(),
+                                              self._enter()))
+        except Exception:
+            self._give(taken)
+            raise
         fresh = [_Sequence(p, n) for p, n in zip(lists, lens)]
         if keep_source:
             out = list(range(self._next, self._next + len(seqs)))
@@ -344,12 +356,8 @@ class PagedKVCache:
         from . import KVCache
         s = self._seq(seq)
         shape = (self.num_heads, s.length, self.head_dim)
-        k = torch.empty(shape, dtype=self.dtype, device=self.keys.device)
-        v = torch.empty(shape, dtype=self.dtype, device=self.keys.device)
-        h = self._plan([s], [0], 0, 0, 0)
-        try:
-            L.check(self._lib.kvf_paged_gather(self._ctx, h, self._pool_ref, self._layer(layer), 0, k.data_ptr(),
-                                               v.data_ptr(), self._enter()))
-        finally:
-            self._lib.kvf_paged_plan_free(h)
+        k, v = self.keys.new_empty(shape), self.keys.new_empty(shape)
+        pages, _ = _ints([s.pages])
+        L.check(self._lib.kvf_paged_gather(self._ctx, self._pool_ref, self._layer(layer), pages, s.length,
+                                           k.data_ptr(), v.data_ptr(), self._enter()))
         return KVCache(k, v, layer)

@@ -689,12 +689,17 @@ def test_refusals(kvf):
     assert lib.kvf_paged_attention(ctx, plan, C.byref(other), 0, q.data_ptr(), 256, 64, 1.0, 0.0, q.data_ptr(), None,
                                    None) == L.ERR_INVALID_CONFIG
     kept = torch.empty(1024, dtype=torch.int32, device="cuda")
-    same = i32(0)
-    assert lib.kvf_paged_evict(ctx, plan, C.byref(c._pool), 1, 0, 0, same.ctypes.data, 1, kept.data_ptr(),
-                               None) == L.ERR_INVALID_CONFIG  # the source's own page
-    assert lib.kvf_paged_evict(ctx, plan, C.byref(other), 1, 0, 0, same.ctypes.data, 1, kept.data_ptr(),
-                               None) == L.ERR_INVALID_CONFIG
-    assert lib.kvf_paged_gather(ctx, plan, C.byref(c._pool), 0, 1, k.data_ptr(), k.data_ptr(),
+    evict = lambda new, pool=c._pool, kv=one, t=tab, stride=1, n=1: lib.kvf_paged_evict(  # noqa: E731
+        ctx, C.byref(pool), n, kv.ctypes.data, t.ctypes.data, stride, 1, 0, 0, new.ctypes.data, 1, kept.data_ptr(),
+        None)
+    assert evict(i32(0)) == L.ERR_INVALID_CONFIG  # the source's own page
+    assert evict(i32(1), pool=other) == L.ERR_INVALID_CONFIG  # no weights
+    assert evict(i32(6)) == L.ERR_SHAPE_MISMATCH and evict(i32(1), t=i32(-1)) == L.ERR_SHAPE_MISMATCH
+    assert evict(i32(1), kv=i32(17)) == L.ERR_SHAPE_MISMATCH and evict(i32(1), kv=i32(-1)) == L.ERR_SHAPE_MISMATCH
+    assert evict(i32(2, 2), kv=i32(1, 1), t=i32(0, 1), n=2) == L.ERR_INVALID_CONFIG  # named twice
+    assert lib.kvf_paged_gather(ctx, C.byref(c._pool), 1, tab.ctypes.data, 1, k.data_ptr(), k.data_ptr(),
+                                None) == L.ERR_SHAPE_MISMATCH
+    assert lib.kvf_paged_gather(ctx, C.byref(c._pool), 0, i32(6).ctypes.data, 1, k.data_ptr(), k.data_ptr(),
                                 None) == L.ERR_SHAPE_MISMATCH
     assert lib.kvf_paged_plan_free(plan) == L.OK and lib.kvf_paged_plan_free(None) == L.OK
     # the codec's entry points do not take bf16
