@@ -1007,11 +1007,9 @@ struct kvf_paged_plan {
   PagedWork weights;  // the same sequences as `slots`, for the tensor-core sums (joins_n 0: none)
   const long long* score_at = nullptr;  // [n] where a sequence's scores start
   size_t scores_n = 0;
-  // workspace: parts of cut tiles (for the largest work list) and their
-  // counters; with weights also the scores, the sums' parts, and the rows' lse
+  // workspace: parts of cut tiles (for the largest work list); with weights also the scores, the sums' parts, and the rows' lse
   float* part_o = nullptr;
   float* part_ml = nullptr;
-  unsigned* counters = nullptr;
   mutable float* scores = nullptr;
   mutable float* part_w = nullptr;
   mutable float* lse = nullptr;
@@ -1209,14 +1207,11 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     }
     for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});
   }
-  size_t parts_floats = 0, parts_rows = 0, joins = 0;
+  size_t parts_floats = 0, parts_rows = 0;
   for (size_t i = 0; i < hosts.size() && i < 2; ++i) {
     parts_rows = std::max(parts_rows, (size_t)hosts[i].parts * hosts[i].row_tile);
     parts_floats = parts_rows * p->dim;
-    joins = std::max(joins, hosts[i].joins.size());
   }
-  const std::vector<unsigned> zeros(joins * kJoinCounters, 0u);
-  const size_t at_counters = img.add(zeros);
   const size_t at_slots = img.add(slots), at_decode_slots = img.add(decode_slots), at_score_at = img.add(score_at);
 
   // one allocation: the image, then the workspace of the parts
@@ -1226,7 +1221,6 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   char* d = static_cast<char*>(p->block);
   p->part_ml = reinterpret_cast<float*>(d + at_ml);
   p->part_o = reinterpret_cast<float*>(d + at_o);
-  p->counters = reinterpret_cast<unsigned*>(d + at_counters);
   p->place = reinterpret_cast<const long long*>(d + at_place);
   p->seqs.table = reinterpret_cast<const int*>(d + at_table);
   p->seqs.stride = max_pages;
@@ -2563,7 +2557,6 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
   a.lse = lse;
   a.part_o = plan->part_o;
   a.part_ml = plan->part_ml;
-  a.counters = plan->counters;
   a.status = ctx->d_status;
   KVF_TRY(plan_enter(plan, st));
   const bool track = decay >= 0.0f;
@@ -2577,15 +2570,14 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
   cudaError_t err = cudaSuccess;
   for (const PagedWork& w : plan->works) {
     if (err != cudaSuccess) break;
-    a.joins = w.joins;
     if (w.kernel == kPagedDecode) {
       err = launch_paged_decode(a, w, track ? plan->scores : nullptr, plan->score_at, st);
     } else if (w.kernel == kPagedChunk) {
       err = launch_paged_chunk(a, w, st);
     } else {
       err = launch_paged_attn_generic(a, w, st);
-      if (err == cudaSuccess) err = launch_paged_join(a, w, st);
     }
+    if (err == cudaSuccess) err = launch_paged_join(a, w, st);
   }
   if (err == cudaSuccess && track && plan->slots_n) {
     err = cudaErrorNotSupported;

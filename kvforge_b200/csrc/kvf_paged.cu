@@ -38,7 +38,8 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
       out->first.push_back((int)out->segs.size());
       left = quota;
     };
-    for (size_t i = 0; i < n; ++i) {
+    int tokens = 0;  // in front of sequence i
+    for (size_t i = 0; i < n; tokens += q_lens[i++]) {
       if (!chosen(i)) continue;
       for (int h = 0; h < heads; ++h)
         for (int r = 0; r < q_lens[i] * group; r += row_tile) {
@@ -50,19 +51,15 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
             if (!fresh && left - fixed < std::min(least, count - it)) close();
             int take = (int)std::min<long long>(count - it, std::max<long long>(left - fixed, 1));
             if (count - it - take < least) take = count - it;  // no sliver behind the cut
-            out->segs.push_back({(int)i, h, r, it, it + take, -1, -1});
+            out->segs.push_back({(int)i, h, r, it, it + take, -1});
             it += take;
             left -= take + fixed;
             if (left <= fixed) close();
           } while (it < count);
           const int parts = (int)(out->segs.size() - seg0);
           if (parts > 1) {
-            for (size_t k = seg0; k < out->segs.size(); ++k) {
-              out->segs[k].part = out->parts + (int)(k - seg0);
-              out->segs[k].join = (int)out->joins.size();
-            }
-            out->joins.push_back({(int)i, h, r, out->parts, parts});
-            out->parts += parts;
+            out->joins.push_back({(int)i, h, r, out->parts, parts, std::min(row_tile, q_lens[i] * group - r), tokens});
+            for (size_t k = seg0; k < out->segs.size(); ++k) out->segs[k].part = out->parts++;
           }
         }
     }

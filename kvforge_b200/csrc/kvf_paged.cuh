@@ -33,13 +33,13 @@ struct PagedSeqs {
 // and an iteration is one tile of `key_tile` slots. One CTA walks the segments
 // [first[cta], first[cta + 1]), each a range of iterations of one row tile. A
 // tile cut into several segments leaves partial results (part >= 0: their
-// slot) that are joined (join: the tile's PagedJoin) by whichever writes the
-// last of them, or afterwards; part = -1 writes the output itself.
+// slot) that are joined afterwards; part = -1 writes the output itself.
 struct PagedSeg {
-  int seq, head, row0, it0, it1, part, join;
+  int seq, head, row0, it0, it1, part;
 };
 struct PagedJoin {
   int seq, head, row0, part0, parts;
+  int rows, token0;  // rows of the tile, first token of the sequence
 };
 // what covers one tile of slots of one sequence (weights): (sequence, first slot)
 struct PagedSlots {
@@ -98,11 +98,8 @@ struct PagedAttn {
   float* lse = nullptr;            // [tokens, heads * group] or nullptr
   float* part_o = nullptr;         // [parts, row_tile, dim] sums before the division
   float* part_ml = nullptr;        // [parts, row_tile, 2] maximum (base 2) and sum
-  const PagedJoin* joins = nullptr;
-  unsigned* counters = nullptr;  // [joins, kJoinCounters] of arrived parts, zero between launches
   unsigned* status = nullptr;
 };
-constexpr int kJoinCounters = 8;
 
 // host side of a work list
 struct PagedWorkHost {
@@ -170,6 +167,24 @@ cudaError_t launch_paged_chunk_weights(const PagedAttn& a, const PagedWork& w, s
                                        float decay, cudaStream_t st);
 
 #ifdef __CUDACC__
+// Launches a kernel that may begin while the one before it in the stream ends:
+// what it does before wait_for_previous() must not depend on that one.
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <typename T>
 __device__ __forceinline__ float to_float(T x);
 template <>

@@ -252,39 +252,59 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const P
   }
 }
 
-// Joins the segments of cut tiles: one warp per row, lanes over the columns.
-constexpr int kJoinWarps = 4;
+// Joins the parts of cut tiles: one warp per row, lanes over the columns. All
+// it needs of the plan is read before it waits for the attention to end, and the
+// first parts' sums and maxima are loaded together; bound by that one latency
+// for short lists, and by reading the parts from L2 for long ones.
+constexpr int kJoinWarps = 4, kJoinAhead = 4;
 template <typename T, int NC>  // NC: columns per lane
 __global__ void __launch_bounds__(32 * kJoinWarps) k_paged_join(PagedAttn a, const PagedJoin* __restrict__ joins,
                                                                 int row_tile) {
   const PagedJoin g = joins[blockIdx.x];
   const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int q0 = __ldg(a.s.q_start + g.seq), nq = __ldg(a.s.q_start + g.seq + 1) - q0;
-  if (r >= min(row_tile, nq * a.group - g.row0)) return;
   const int D = a.c.dim;
-  const float* ml = a.part_ml + ((size_t)g.part0 * row_tile + r) * 2;
-  float m = -INFINITY;
-  for (int p = lane; p < g.parts; p += 32) m = fmaxf(m, __ldg(ml + (size_t)p * row_tile * 2));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[NC];
+  wait_for_previous();
+  if (r >= g.rows) return;
+  const size_t row = (size_t)g.part0 * row_tile + r;
+  const float* ml = a.part_ml + row * 2;
+  const float* po = a.part_o + row * D;
+  float m = -INFINITY, l = 0.0f, acc[NC];
 #pragma unroll
   for (int u = 0; u < NC; ++u) acc[u] = 0.0f;
-  const float* po = a.part_o + ((size_t)g.part0 * row_tile + r) * D;
-#pragma unroll 4
-  for (int p = 0; p < g.parts; ++p) {
-    const float2 x = *reinterpret_cast<const float2*>(ml + (size_t)p * row_tile * 2);
-    const float w = exp2f(x.x - mu);
-    l = fmaf(w, x.y, l);
+  // as in the attention itself, over parts instead of tiles
+  for (int p0 = 0; p0 < g.parts; p0 += kJoinAhead) {
+    float2 y[kJoinAhead];
+    float x[kJoinAhead][NC];
 #pragma unroll
-    for (int u = 0; u < NC; ++u) {
-      const int c = lane + 32 * u;
-      if (c < D) acc[u] = fmaf(w, __ldg(po + (size_t)p * row_tile * D + c), acc[u]);
+    for (int k = 0; k < kJoinAhead; ++k) {
+      const size_t at = (size_t)(p0 + k) * row_tile;
+      y[k] = make_float2(-INFINITY, 0.0f);
+      if (p0 + k < g.parts) y[k] = *reinterpret_cast<const float2*>(ml + at * 2);
+#pragma unroll
+      for (int u = 0; u < NC; ++u) {
+        x[k][u] = 0.0f;
+        if (p0 + k < g.parts && lane + 32 * u < D) x[k][u] = po[at * D + lane + 32 * u];
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k) top = fmaxf(top, y[k].x);
+    const float mu = top == -INFINITY ? 0.0f : top, f = exp2f(m - mu);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int u = 0; u < NC; ++u) acc[u] *= f;
+#pragma unroll
+    for (int k = 0; k < kJoinAhead; ++k) {
+      if (p0 + k >= g.parts) continue;
+      const float w = exp2f(y[k].x - mu);
+      l = fmaf(w, y[k].y, l);
+#pragma unroll
+      for (int u = 0; u < NC; ++u) acc[u] = fmaf(w, x[k][u], acc[u]);
     }
   }
   const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
-  const size_t at = (size_t)(q0 + t) * (a.c.heads * a.group) + hq;
+  const size_t at = (size_t)(g.token0 + t) * (a.c.heads * a.group) + hq;
   const bool none = l == 0.0f;
   if (lane == 0 && a.lse) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * (float)M_LN2;
   const float inv = none ? 0.0f : 1.0f / l;
@@ -404,11 +424,9 @@ cudaError_t attn_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) 
 template <typename T>
 cudaError_t join_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
   const dim3 grid((unsigned)w.joins_n, (unsigned)((w.row_tile + kJoinWarps - 1) / kJoinWarps));
-  if (a.c.dim <= 64) k_paged_join<T, 2><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
-  else if (a.c.dim <= 128) k_paged_join<T, 4><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
-  else k_paged_join<T, 8><<<grid, 32 * kJoinWarps, 0, st>>>(a, w.joins, w.row_tile);
   note_launches(1);
-  return cudaGetLastError();
+  auto kern = a.c.dim <= 64 ? k_paged_join<T, 2> : a.c.dim <= 128 ? k_paged_join<T, 4> : k_paged_join<T, 8>;
+  return launch_behind(kern, grid, 32 * kJoinWarps, 0, st, a, w.joins, w.row_tile);
 }
 
 template <typename T, int RT>

@@ -543,20 +543,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (a.lse)
           a.lse[at] = none ? -INFINITY : (m2 + log2f(l)) * (float)M_LN2;
       }
-      if (s.g.part >= 0) {
-        // the 32 rows of this warp, by the warp that brings their last part
-        const PagedJoin j = a.joins[s.g.join];
-        if (last_part(a.counters + s.g.join * kJoinCounters + w, j.parts)) {
-          const int r0 = 32 * w, r1 = min(s.rows, r0 + 32);
-#pragma unroll 2
-          for (int k = r0; k < r1; ++k) {
-            const int tk = (s.g.row0 + k) / a.group, hk = s.g.head * a.group + (s.g.row0 + k) % a.group;
-            const size_t out = (size_t)(s.q0 + tk) * (a.c.heads * a.group) + hk, row = (size_t)j.part0 * kRows + k;
-            join_row<T, DP / 32>(a.part_ml + row * 2, a.part_o + row * D, j.parts, kRows, D, lane, D,
-                                 static_cast<T*>(a.out) + out * D, a.lse ? a.lse + out : nullptr);
-          }
-        }
-      }
       ring0 += 2 * count;  // (only the first row tile, which every segment has, uses it)
       // the next segment's products overwrite O: ordered by its numerators' barrier
       fence_before();

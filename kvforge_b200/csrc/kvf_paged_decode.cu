@@ -37,7 +37,7 @@ template <int DP>
 constexpr int tile_bytes() { return kKeys * DP * 2; }
 // a segment as the producer hands it to the consumers
 struct Head {
-  int seq, head, row0, it0, it1, part, join, n, nq, q0;
+  int seq, head, row0, it0, it1, part, n, nq, q0;
 };
 constexpr int kPStride = kKeys + 8;  // numerators of a row, 16-bit: eight rows apart lie in different banks
 template <int DP>
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (si < seg1) {
         const PagedSeg g = segs[si];
         const int q0 = __ldg(a.s.q_start + g.seq);
-        d = {g.seq, g.head, g.row0, g.it0, g.it1, g.part, g.join, __ldg(a.s.kv_len + g.seq),
+        d = {g.seq, g.head, g.row0, g.it0, g.it1, g.part, __ldg(a.s.kv_len + g.seq),
              __ldg(a.s.q_start + g.seq + 1) - q0, q0};
       }
       return d;
@@ -428,26 +428,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (g.part >= 0) a.part_o[((size_t)g.part * kRows + r) * D + col] = v;
             else static_cast<T*>(a.out)[at * D + col] = from_float<T>(none ? 0.0f : v * inv);
           }
-        if ((lane & 3) == 0) {
-          // (every warp writes the same, so that each may join its columns by itself)
+        if (w == 0 && (lane & 3) == 0) {
           if (g.part >= 0)
             *reinterpret_cast<float2*>(a.part_ml + ((size_t)g.part * kRows + r) * 2) = make_float2(m[i], L);
-          else if (w == 0 && a.lse)
+          else if (a.lse)
             a.lse[at] = none ? -INFINITY : (m[i] + log2f(L)) * (float)M_LN2;
-        }
-      }
-      if (g.part >= 0) {
-        const PagedJoin j = a.joins[g.join];
-        if (last_part(a.counters + g.join * kJoinCounters + w, j.parts)) {
-          const int c = 8 * kCols * w + lane, cols = min(D, 8 * kCols * (w + 1));
-#pragma unroll 2
-          for (int r = 0; r < rows; ++r) {
-            const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
-            const size_t at = (size_t)(g.q0 + t) * Hq + hq;
-            const size_t row = (size_t)j.part0 * kRows + r;
-            join_row<T, 1>(a.part_ml + row * 2, a.part_o + row * D, j.parts, kRows, D, c, cols,
-                           static_cast<T*>(a.out) + at * D, w == 0 && a.lse ? a.lse + at : nullptr);
-          }
         }
       }
     }
@@ -466,6 +451,7 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAt
   const PagedSlots g = tiles[blockIdx.x];
   const int h = blockIdx.y, n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
   const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = nq * a.group;
+  wait_for_previous();
   if ((int)threadIdx.x < rows) {
     const int t = threadIdx.x / a.group, hq = h * a.group + threadIdx.x % a.group;
     lse2[threadIdx.x] = a.lse[(size_t)(q0 + t) * (a.c.heads * a.group) + hq] * (float)M_LOG2E;
@@ -523,10 +509,9 @@ cudaError_t launch_paged_decode(const PagedAttn& a, const PagedWork& w, float* s
 cudaError_t launch_paged_decode_weights(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles,
                                         const float* scores, const long long* score_at, float decay, cudaStream_t st) {
   if (ntiles == 0) return cudaSuccess;
-  k_paged_decode_weights<<<dim3((unsigned)ntiles, (unsigned)a.c.heads), kWeightThreads, 0, st>>>(a, tiles, scores,
-                                                                                                score_at, decay);
   note_launches(1);
-  return cudaGetLastError();
+  return launch_behind(k_paged_decode_weights, dim3((unsigned)ntiles, (unsigned)a.c.heads), kWeightThreads, 0, st, a,
+                       tiles, scores, score_at, decay);
 }
 
 }  // namespace kvf

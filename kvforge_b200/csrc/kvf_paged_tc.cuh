@@ -207,55 +207,6 @@ __device__ __forceinline__ bool drop_nonfinite(uint4& w) {
   }
   return any;
 }
-// Counts this warp's part of a cut tile (every lane's stores before the call);
-// true on the warp that brings the last of them, which then joins them. The
-// counter is back at zero afterwards.
-__device__ __forceinline__ bool last_part(unsigned* counter, int parts) {
-  __threadfence();
-  __syncwarp();
-  unsigned old = 0;
-  if ((threadIdx.x & 31) == 0) {
-    old = atomicAdd(counter, 1u);
-    if (old == (unsigned)parts - 1) *counter = 0;
-  }
-  old = __shfl_sync(0xffffffffu, old, 0);
-  if (old != (unsigned)parts - 1) return false;
-  __threadfence();
-  return true;
-}
-
-// One row of a cut tile from its parts: sum_p w_p O_p / sum_p w_p l_p with w_p =
-// 2^(m_p - max m), in the order of the parts whichever warp does it. `stride`
-// rows between parts; lane's columns c, c + 32, ... below `cols` (NC of them);
-// ml and o point at the row's first part.
-template <typename T, int NC>
-__device__ __forceinline__ void join_row(const float* ml, const float* o, int parts, size_t stride, int D, int c,
-                                         int cols, T* out, float* lse) {
-  const int lane = threadIdx.x & 31;
-  float m = -INFINITY;
-  for (int p = lane; p < parts; p += 32) m = fmaxf(m, __ldcg(ml + p * stride * 2));
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, acc[NC];
-#pragma unroll
-  for (int u = 0; u < NC; ++u) acc[u] = 0.0f;
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(ml + p * stride * 2));
-    const float w = ptx::ex2(x.x - mu);
-    l = fmaf(w, x.y, l);
-#pragma unroll
-    for (int u = 0; u < NC; ++u)
-      if (c + 32 * u < cols) acc[u] = fmaf(w, __ldcg(o + p * stride * D + c + 32 * u), acc[u]);
-  }
-  const bool none = l == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int u = 0; u < NC; ++u)
-    if (c + 32 * u < cols) out[c + 32 * u] = from_float<T>(none ? 0.0f : acc[u] * inv);
-  if (lse && lane == 0) *lse = none ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
-}
 #endif
 
 }  // namespace kvf

@@ -77,12 +77,12 @@ void paged_split_slots(const int* q_lens, const int* kv_lens, size_t n, int head
             if (left - kFixed < std::min(4, t1 - t0) && left < quota) close();
             int take = (int)std::min<long long>(t1 - t0, std::max<long long>(left - kFixed, 1));
             if (t1 - t0 - take < 4) take = t1 - t0;
-            out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++, -1});
+            out->segs.push_back({(int)i, h, j, t0, t0 + take, out->parts++});
             t0 += take;
             left -= take + kFixed;
             if (left <= kFixed) close();
           }
-          out->joins.push_back({(int)i, h, j, part0, out->parts - part0});
+          out->joins.push_back({(int)i, h, j, part0, out->parts - part0, 0, 0});
         }
     }
     close();
@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they start at 0
   const int seg0 = __ldg(first + blockIdx.x), seg1 = __ldg(first + blockIdx.x + 1);
   bool gave_up = false;
+  wait_for_previous();  // lse
 
   if (w == kSumWarps) {
     // ---------------- loads ----------------
@@ -372,7 +373,9 @@ __global__ void __launch_bounds__(kWeightSlots) k_paged_chunk_weights_join(Paged
                                                                            float decay) {
   const PagedJoin g = joins[blockIdx.x];
   const int j = g.row0 + threadIdx.x;
-  if (j >= __ldg(a.s.kv_len + g.seq)) return;
+  const bool there = j < __ldg(a.s.kv_len + g.seq);
+  wait_for_previous();
+  if (!there) return;
   float t = 0.0f;
 #pragma unroll 4
   for (int p = 0; p < 2 * g.parts; ++p) t += __ldg(part_w + ((size_t)2 * g.part0 + p) * kWeightSlots + threadIdx.x);
@@ -404,9 +407,8 @@ cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& qm, const Pag
   constexpr size_t bytes = smem_bytes<DP>();
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  kern<<<w.ctas, kThreads, bytes, st>>>(km, qm, a, w.segs, w.first, part_w);
   note_launches(1);
-  return cudaGetLastError();
+  return launch_behind(kern, dim3(w.ctas), kThreads, bytes, st, km, qm, a, w.segs, w.first, part_w);
 }
 
 }  // namespace
@@ -426,9 +428,8 @@ cudaError_t launch_paged_chunk_weights(const PagedAttn& a, const PagedWork& w, s
                         : launch_typed<__nv_bfloat16, 128>(km, qm, a, w, part_w, st);
   }
   if (e != cudaSuccess || w.joins_n == 0) return e;
-  k_paged_chunk_weights_join<<<w.joins_n, kWeightSlots, 0, st>>>(a, w.joins, part_w, decay);
   note_launches(1);
-  return cudaGetLastError();
+  return launch_behind(k_paged_chunk_weights_join, dim3(w.joins_n), kWeightSlots, 0, st, a, w.joins, part_w, decay);
 }
 
 }  // namespace kvf
