@@ -25,6 +25,9 @@ constexpr int kPStride = kGenKeys + 4;  // rows of P, 16-byte aligned, four bank
 // at one column lie in different banks
 __device__ __forceinline__ int tile_at(int r, int c4, int DP) { return r * DP + ((c4 ^ (r & 7)) << 2); }
 
+__device__ float4 g_zero;
+__device__ __forceinline__ const void* sm_zero() { return &g_zero; }
+
 // four (f32) or eight (16-bit) elements of a row as floats
 template <typename T>
 __device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
@@ -35,25 +38,42 @@ __device__ __forceinline__ void load16(const T* p, float (&x)[16 / sizeof(T)]) {
 }
 
 // Fills `rows` rows of DP floats; row(r) points at row r's first element, or
-// is nullptr for a row of zeros.
+// is nullptr for a row of zeros. Rows of f32 in 16-byte pieces are copied
+// asynchronously: one group, committed here; everything else is there at once.
 template <typename T, typename Row>
 __device__ __forceinline__ void fill_tile(float* sm, int rows, int DP, int D, bool wide, Row row) {
   if (wide) {
     constexpr int E = 16 / sizeof(T);
-    const int per = DP / E;
+    // piece i = (r, c): i grows by the block's threads, without a division
+    const int per = DP / E, dr = kGenThreads / per, dc = kGenThreads - dr * per;
+    int r = threadIdx.x / per, c = threadIdx.x - r * per;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < rows * per; i += kGenThreads) {
-      const int r = i / per, c = (i - r * per) * E;
+    while (r < rows) {
       const T* p = row(r);
-      float x[E];
-      if (p && c < D) load16(p + c, x);
-      else
+      const bool there = p && c * E < D;
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(sm + tile_at(r, c, DP));
+        // (a piece of zero bytes is filled with zeros; its address is any valid one)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                     "l"(there ? (const void*)(p + c * E) : (const void*)sm_zero()), "r"(there ? 16 : 0)
+                     : "memory");
+      } else {
+        float x[E];
+        if (there) load16(p + c * E, x);
+        else
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = 0.0f;
+          for (int e = 0; e < E; ++e) x[e] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<float4*>(sm + tile_at(r, (c + e) >> 2, DP)) =
-            make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(sm + tile_at(r, (c * E + e) >> 2, DP)) =
+              make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      }
+      r += dr;
+      c += dc;
+      if (c >= per) {
+        c -= per;
+        ++r;
+      }
     }
   } else {
     for (int i = threadIdx.x; i < rows * DP; i += kGenThreads) {
@@ -62,6 +82,12 @@ __device__ __forceinline__ void fill_tile(float* sm, int rows, int DP, int D, bo
       sm[tile_at(r, c >> 2, DP) + (c & 3)] = (p && c < D) ? to_float(p[c]) : 0.0f;
     }
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+// waits until at most N of this thread's groups are still on their way
+template <int N>
+__device__ __forceinline__ void filled() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // scores of RT rows (ty * RT + i) and four slots (tx + 16 u) of this thread
@@ -106,18 +132,17 @@ __device__ __forceinline__ float half_sum(float v) {
 // rows and four slots, then those rows' sums of NU groups of four columns.
 // Tiles of 64 slots; 64 rows (RT = 4) where there are many, 16 (RT = 1) for
 // single tokens. Bound by the CUDA cores' multiply-adds at 64 rows and by
-// loads at 16, where two or three CTAs share an SM so that one loads while
-// another computes.
+// loads at 16; two CTAs (64 rows, head_dim 128: 113 KB each) or three share an SM.
 template <typename T, int RT, int NU>
-__global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const PagedSeg* __restrict__ segs,
+__global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(PagedAttn a, const PagedSeg* __restrict__ segs,
                                                             const int* __restrict__ first, int DP, bool wide,
                                                             bool wide_q) {
   constexpr int BR = 16 * RT;
   extern __shared__ float4 sm4[];
   float* Q = reinterpret_cast<float*>(sm4);  // [BR][DP]
-  float* K = Q + BR * DP;                    // [64][DP]
-  float* V = K + kGenKeys * DP;              // [64][DP]
-  float* P = V + kGenKeys * DP;              // [BR][kPStride]
+  float* V = Q + BR * DP;                    // [64][DP]
+  float* K = V + kGenKeys * DP;              // [64][DP]
+  float* P = K + kGenKeys * DP;              // [BR][kPStride]
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int D = a.c.dim, Hq = a.c.heads * a.group;
   const int s1 = __ldg(first + blockIdx.x + 1);
@@ -134,33 +159,42 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const P
       return static_cast<const T*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
     });
     int pos[RT];
-    float m[RT], l[RT], o[RT][NU][4];
+    float m[RT], l[RT];
+    float2 o[RT][NU][2];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       pos[i] = n - nq + (g.row0 + ty * RT + i) / a.group;
       m[i] = -INFINITY;
       l[i] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][u][e] = 0.0f;
+      for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = make_float2(0.0f, 0.0f);
     }
     const int pa = n - nq + g.row0 / a.group, pb = n - nq + (g.row0 + rows - 1) / a.group;
-    for (int it = g.it0; it < g.it1; ++it) {
-      const int j0 = (it < span.nsink ? it : span.first + it - span.nsink) * kGenKeys;
-      __syncthreads();
-      // slots that no row of the tile sees (past the last one, between the
-      // sinks and the window) are zeros here, whatever their pages hold
-      auto slot = [&](const void* pool, int r) -> const T* {
+    auto slot0 = [&](int it) { return (it < span.nsink ? it : span.first + it - span.nsink) * kGenKeys; };
+    // slots that no row of the tile sees (past the last one, between the sinks
+    // and the window) are zeros here, whatever their pages hold
+    auto fill = [&](float* to, const void* pool, int it) {
+      const int j0 = slot0(it);
+      fill_tile<T>(to, kGenKeys, DP, D, wide, [&](int r) -> const T* {
         const int j = j0 + r;
         if (j > pb || (a.window && j <= pa - a.window && j >= a.sinks)) return nullptr;
         return static_cast<const T*>(pool) + paged_row(table, a.c, g.head, j);
-      };
-      fill_tile<T>(K, kGenKeys, DP, D, wide, [&](int r) { return slot(a.c.keys, r); });
-      fill_tile<T>(V, kGenKeys, DP, D, wide, [&](int r) { return slot(a.c.values, r); });
+      });
+    };
+    // K of the next tile is on its way while the values are summed, V of the
+    // next one while its scores are computed
+    if (g.it0 < g.it1) {
+      fill(K, a.c.keys, g.it0);
+      fill(V, a.c.values, g.it0);
+    }
+    for (int it = g.it0; it < g.it1; ++it) {
+      const int j0 = slot0(it);
+      filled<1>();
       __syncthreads();
       float s[RT][4];
       scores<RT>(Q, K, DP, ty, tx, s);
+      __syncthreads();  // K is read
+      if (it + 1 < g.it1) fill(K, a.c.keys, it + 1);
       // a tile that every row sees whole needs no masks
       const bool whole = j0 + kGenKeys - 1 <= pa &&
                          (!a.window || j0 > pb - a.window || j0 + kGenKeys <= a.sinks);
@@ -191,9 +225,14 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const P
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][u][e] *= f;
+          for (int e = 0; e < 2; ++e) {
+            o[i][u][e].x *= f;
+            o[i][u][e].y *= f;
+          }
       }
-      __syncwarp();  // the rows of P that this half-warp wrote are its own
+      if (it + 1 < g.it1) filled<1>();
+      else filled<0>();
+      __syncthreads();  // V is there (the rows of P that a half-warp reads are its own)
       auto accumulate = [&](auto masked) {
 #pragma unroll 1
         for (int k4 = 0; k4 < kGenKeys; k4 += 4) {
@@ -211,16 +250,19 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const P
               for (int i = 0; i < RT; ++i) {
                 const float pk = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
                 if (decltype(masked)::value && pk < 0.0f) continue;
-                o[i][u][0] = fmaf(pk, v.x, o[i][u][0]);
-                o[i][u][1] = fmaf(pk, v.y, o[i][u][1]);
-                o[i][u][2] = fmaf(pk, v.z, o[i][u][2]);
-                o[i][u][3] = fmaf(pk, v.w, o[i][u][3]);
+                const float2 p2 = make_float2(pk, pk);
+                o[i][u][0] = ffma2(p2, make_float2(v.x, v.y), o[i][u][0]);
+                o[i][u][1] = ffma2(p2, make_float2(v.z, v.w), o[i][u][1]);
               }
             }
         }
       };
       if (whole) accumulate(std::false_type{});
       else accumulate(std::true_type{});
+      if (it + 1 < g.it1) {
+        __syncthreads();  // V is read
+        fill(V, a.c.values, it + 1);
+      }
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -245,8 +287,9 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_attn(PagedAttn a, const P
         for (int e = 0; e < 4; ++e) {
           const int c = 4 * (tx + 16 * u) + e;
           if (c >= D) continue;
-          if (g.part >= 0) a.part_o[((size_t)g.part * BR + r) * D + c] = o[i][u][e];
-          else static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : o[i][u][e] * inv);
+          const float x = e & 1 ? o[i][u][e >> 1].y : o[i][u][e >> 1].x;
+          if (g.part >= 0) a.part_o[((size_t)g.part * BR + r) * D + c] = x;
+          else static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : x * inv);
         }
     }
   }
@@ -354,6 +397,7 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_weights(PagedAttn a, cons
       const int t = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
       lse2[r] = a.lse[(size_t)(q0 + t) * Hq + hq] * (float)M_LOG2E;
     }
+    filled<0>();
     __syncthreads();
     float s[RT][4];
     scores<RT>(Q, K, DP, ty, tx, s);
