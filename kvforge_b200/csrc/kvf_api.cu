@@ -1202,7 +1202,7 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
       for (int j = 0; j < kv_lens[i]; j += step) (decode ? decode_slots : slots).push_back({(int)i, j});
       if (decode) {
         score_at[i] = (long long)p->scores_n;
-        p->scores_n += (size_t)heads * q_lens[i] * group * kv_lens[i];
+        p->scores_n += (size_t)heads * q_lens[i] * group * ((kv_lens[i] + 3) & ~3);
       }
     }
     for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});

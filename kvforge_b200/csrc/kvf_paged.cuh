@@ -3,6 +3,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <vector>
 
 #include "kvf_internal.cuh"
@@ -167,6 +168,23 @@ cudaError_t launch_paged_chunk_weights(const PagedAttn& a, const PagedWork& w, s
                                        float decay, cudaStream_t st);
 
 #ifdef __CUDACC__
+// Opts a kernel in to `bytes` of dynamic shared memory, once per device (each
+// call site passes flags of its own; the same whichever thread sets them).
+struct OptInOnce {
+  static constexpr int kDevices = 64;
+  std::atomic<size_t> bytes[kDevices];
+};
+template <typename K>
+cudaError_t opt_in_once(OptInOnce& done, K kern, size_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= OptInOnce::kDevices) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+  if (done.bytes[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.bytes[dev].store(bytes, std::memory_order_release);
+  return e;
+}
+
 // Launches a kernel that may begin while the one before it in the stream ends:
 // what it does before wait_for_previous() must not depend on that one.
 template <typename... P, typename... A>

@@ -562,7 +562,8 @@ cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& vm, const Pag
                          cudaStream_t st) {
   auto kern = k_paged_chunk<T, DP>;
   constexpr size_t bytes = smem_bytes<DP>();
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, bytes);
   if (e != cudaSuccess) return e;
   const bool wide_q = (a.q_token | a.q_head) % 8 == 0 && aligned(a.q, 16);
   kern<<<w.ctas, kThreads, bytes, st>>>(km, vm, a, w.segs, w.first, wide_q, aligned(a.out, 16));

@@ -120,7 +120,8 @@ __device__ __noinline__ float nonfinite_sum(const T* v, const int* table, int sh
 }
 
 // scores != nullptr: every score (base 2, -inf where unseen) is also written,
-// for the attention weights: sequence i's at scores + score_at[i], [head][row][slot]
+// for the attention weights: sequence i's at scores + score_at[i], [head][row][slot],
+// rows of a multiple of four slots
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 2)
     k_paged_decode(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttn a,
@@ -269,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int c = 0; c < kCols; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
-      float* sc = scores ? scores + score_at[g.seq] + ((size_t)g.head * g.nq * a.group + g.row0) * g.n : nullptr;
+      const size_t sc_row = (size_t)((g.n + 3) & ~3);
+      float* sc = scores ? scores + score_at[g.seq] + ((size_t)g.head * g.nq * a.group + g.row0) * sc_row : nullptr;
       bool stop = false;
 
       for (int it = g.it0; it < g.it1; ++it) {
@@ -303,13 +305,14 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (!whole && !paged_sees(pos[e >> 1], j0 + 8 * t + c0 + (e & 1), a.window, a.sinks)) x[t][e] = -INFINITY;
             mx[e >> 1] = fmaxf(mx[e >> 1], x[t][e]);
           }
-        if (sc) {
+        if (sc) {  // pairs of slots: a row's padding takes the one past its end
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = r0 + 8 * (e >> 1), j = j0 + 8 * t + c0 + (e & 1);
-              if (r < rows && j < g.n) sc[(size_t)r * g.n + j] = x[t][e];
+            for (int i = 0; i < 2; ++i) {
+              const int r = r0 + 8 * i, j = j0 + 8 * t + c0;
+              if (r < rows && j < g.n)
+                *reinterpret_cast<float2*>(sc + r * sc_row + j) = make_float2(x[t][2 * i], x[t][2 * i + 1]);
             }
         }
 #pragma unroll
@@ -440,42 +443,65 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (gave_up && a.status) atomicOr(a.status, kDevErrTimeout);
 }
 
-// Attention weights from the scores that k_paged_decode wrote: a thread per
-// slot adds its rows in order.
-constexpr int kWeightThreads = kDecodeWeightSlots;
+// Attention weights from the scores that k_paged_decode wrote: a thread adds
+// four slots' rows in order, 64 threads a (tile, head), the loads of eight rows
+// in flight. Bound by reading the scores, mostly from L2.
+constexpr int kWeightThreads = 256;
+constexpr int kWeightHeads = kWeightThreads * 4 / kDecodeWeightSlots;
 __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,
                                                                          const float* __restrict__ scores,
                                                                          const long long* __restrict__ score_at,
                                                                          float decay) {
-  __shared__ float lse2[kRows];
+  __shared__ float lse2[kWeightHeads][kRows];
   const PagedSlots g = tiles[blockIdx.x];
-  const int h = blockIdx.y, n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+  const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
   const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = nq * a.group;
-  wait_for_previous();
-  if ((int)threadIdx.x < rows) {
-    const int t = threadIdx.x / a.group, hq = h * a.group + threadIdx.x % a.group;
-    lse2[threadIdx.x] = a.lse[(size_t)(q0 + t) * (a.c.heads * a.group) + hq] * (float)M_LOG2E;
-  }
-  __syncthreads();
-  const int j = g.slot0 + threadIdx.x;
-  if (j >= n) return;
+  const int hs = threadIdx.x / (kDecodeWeightSlots / 4), h = blockIdx.y * kWeightHeads + hs;
+  const int j = g.slot0 + 4 * (threadIdx.x % (kDecodeWeightSlots / 4));
   // tiles that no row visits were not written
   const PagedSpan span = paged_span(0, kRows, a.group, n, nq, a.window, a.sinks, kKeys);
   const int tile = j / kKeys;
   const bool there = tile < span.nsink || (tile >= span.first && tile < span.first + span.count - span.nsink);
-  float t = 0.0f;
+  const size_t sc_row = (size_t)((n + 3) & ~3);
+  const float* sc = scores + score_at[g.seq] + (size_t)h * rows * sc_row + j;
+  wait_for_previous();
+  if ((int)threadIdx.x < kWeightHeads * kRows) {
+    const int r = threadIdx.x % kRows, hl = blockIdx.y * kWeightHeads + threadIdx.x / kRows;
+    float z = INFINITY;  // a row that is not there, or sees nothing, adds 0
+    if (r < rows && hl < a.c.heads) {
+      z = a.lse[(size_t)(q0 + r / a.group) * (a.c.heads * a.group) + hl * a.group + r % a.group] * (float)M_LOG2E;
+      if (z == -INFINITY) z = INFINITY;
+    }
+    lse2[threadIdx.x / kRows][r] = z;
+  }
+  __syncthreads();
+  if (h >= a.c.heads || j >= n) return;
+  float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (there) {
-    const float* sc = scores + score_at[g.seq] + (size_t)h * rows * n + j;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      const float z = lse2[r];
-      const float p = exp2f(__ldg(sc + (size_t)r * n) - z);
-      t += z == -INFINITY ? 0.0f : p;
+#pragma unroll
+    for (int r0 = 0; r0 < kRows; r0 += 8) {
+      if (r0 >= rows) break;
+      float4 x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r0 + r < rows) x[r] = __ldg(reinterpret_cast<const float4*>(sc + (r0 + r) * sc_row));
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r0 + r >= rows) continue;
+        const float z = lse2[hs][r0 + r];
+        t[0] += exp2f(x[r].x - z);
+        t[1] += exp2f(x[r].y - z);
+        t[2] += exp2f(x[r].z - z);
+        t[3] += exp2f(x[r].w - z);
+      }
     }
   }
+  // four slots lie in one page
   const int page = __ldg(a.s.table + (size_t)g.seq * a.s.stride + (j >> a.c.page_shift));
   float* p = a.c.weights + (((size_t)page * a.c.heads + h) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
-  *p = decay == 0.0f ? t : fmaf(decay, *p, t);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < n) p[e] = decay == 0.0f ? t[e] : fmaf(decay, p[e], t[e]);
 }
 
 template <typename T, int DP>
@@ -483,7 +509,8 @@ cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& vm, const Pag
                          float* scores, const long long* score_at, cudaStream_t st) {
   auto kern = k_paged_decode<T, DP>;
   constexpr size_t smem = smem_bytes<DP>();
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, smem);
   if (e != cudaSuccess) return e;
   const bool wide_q = (a.q_token | a.q_head) % 8 == 0 && aligned(a.q, 16);
   kern<<<w.ctas, kThreads, smem, st>>>(km, vm, a, w.segs, w.first, scores, score_at, wide_q);
@@ -510,7 +537,7 @@ cudaError_t launch_paged_decode_weights(const PagedAttn& a, const PagedSlots* ti
                                         const float* scores, const long long* score_at, float decay, cudaStream_t st) {
   if (ntiles == 0) return cudaSuccess;
   note_launches(1);
-  return launch_behind(k_paged_decode_weights, dim3((unsigned)ntiles, (unsigned)a.c.heads), kWeightThreads, 0, st, a,
+  return launch_behind(k_paged_decode_weights, dim3((unsigned)ntiles, (unsigned)((a.c.heads + kWeightHeads - 1) / kWeightHeads)), kWeightThreads, 0, st, a,
                        tiles, scores, score_at, decay);
 }
 

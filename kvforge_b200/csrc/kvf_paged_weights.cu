@@ -405,7 +405,8 @@ cudaError_t launch_typed(const CUtensorMap& km, const CUtensorMap& qm, const Pag
                          float* part_w, cudaStream_t st) {
   auto kern = k_paged_chunk_weights<T, DP>;
   constexpr size_t bytes = smem_bytes<DP>();
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, bytes);
   if (e != cudaSuccess) return e;
   note_launches(1);
   return launch_behind(kern, dim3(w.ctas), kThreads, bytes, st, km, qm, a, w.segs, w.first, part_w);
