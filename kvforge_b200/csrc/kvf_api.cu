@@ -1160,39 +1160,43 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
 
   struct Offsets { size_t segs, first, joins; };
   std::vector<Offsets> at;
-  std::vector<PagedWorkHost> hosts;
+  std::vector<PagedWorkHost> hosts;  // the attention's, then (weights_host) the weights'
+  size_t weights_host = SIZE_MAX;
   std::vector<PagedSlots> slots, decode_slots;
   std::vector<long long> score_at;
   if (query_heads && tokens) {
     int sms = 0;
     KVF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device));
     const int group = (int)p->group, heads = (int)p->heads;
-    hosts.resize(2);
     const bool tc = paged_tc_fits(p->dtype, p->dim);
-    const long long few = kDecodeRows;
+    const long long few = kDecodeRows, most = (long long)kMaxLen;
     static_assert(kDecodeRows == kGenRowsShort, "the same sequences have few rows for both kernels");
+    // sequences of lo..hi rows per KV head; CTAs at once; shortest segment; what
+    // a segment's start and end cost, in tiles
+    auto add = [&](int kernel, long long lo, long long hi, int row_tile, int key_tile, int ctas, int least, int fixed) {
+      PagedWorkHost h;
+      h.kernel = kernel;
+      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, lo, hi, row_tile, key_tile, ctas, least, fixed,
+                  &h);
+      if (!h.segs.empty()) hosts.push_back(std::move(h));
+    };
     if (tc) {
-      // two CTAs per SM; a segment's start and end cost about five tiles of loads
-      hosts[0].kernel = kPagedDecode;
-      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kDecodeRows, kDecodeKeys, 2 * sms, 2, 5,
-                  &hosts[0]);
+      add(kPagedDecode, 1, few, kDecodeRows, kDecodeKeys, 2 * sms, 2, 5);
+      add(kPagedChunk, few + 1, most, kChunkRows, kChunkKeys, sms, 4, 2);
     } else {
-      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1,
-                  &hosts[0]);
+      add(kPagedGeneric, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1);
+      add(kPagedGeneric, few + 1, most, kGenRows, kGenKeys, 2 * sms, 2, 1);
     }
-    if (tc) {
-      // one CTA per SM; a segment's start and end cost about two tiles
-      hosts[1].kernel = kPagedChunk;
-      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kChunkRows,
-                  kChunkKeys, sms, 4, 2, &hosts[1]);
-    } else {
-      paged_split(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few + 1, (long long)kMaxLen, kGenRows, kGenKeys,
-                  2 * sms, 2, 1, &hosts[1]);
-    }
-    p->few_rows = hosts[1].segs.empty();
+    p->few_rows = true;
+    for (size_t i = 0; i < n; ++i)
+      if ((long long)q_lens[i] * group > few) p->few_rows = false;
     if (tc && group <= 128) {
-      hosts.resize(3);
-      paged_split_slots(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few, sms, &hosts[2]);
+      PagedWorkHost h;
+      paged_split_slots(q_lens, kv_lens, n, heads, group, p->window, p->sinks, few, sms, &h);
+      if (!h.joins.empty()) {
+        weights_host = hosts.size();
+        hosts.push_back(std::move(h));
+      }
     }
     score_at.assign(n, 0);
     for (size_t i = 0; i < n; ++i) {
@@ -1208,7 +1212,8 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     for (const auto& h : hosts) at.push_back({img.add(h.segs), img.add(h.first), img.add(h.joins)});
   }
   size_t parts_floats = 0, parts_rows = 0;
-  for (size_t i = 0; i < hosts.size() && i < 2; ++i) {
+  for (size_t i = 0; i < hosts.size(); ++i) {
+    if (i == weights_host) continue;
     parts_rows = std::max(parts_rows, (size_t)hosts[i].parts * hosts[i].row_tile);
     parts_floats = parts_rows * p->dim;
   }
@@ -1229,7 +1234,6 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   p->seqs.n = (int)n;
   for (size_t i = 0; i < hosts.size(); ++i) {
     const PagedWorkHost& h = hosts[i];
-    if (h.segs.empty() && h.joins.empty()) continue;
     PagedWork w;
     w.kernel = h.kernel;
     w.row_tile = h.row_tile;
@@ -1241,7 +1245,7 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     w.segs = reinterpret_cast<const PagedSeg*>(d + at[i].segs);
     w.first = reinterpret_cast<const int*>(d + at[i].first);
     w.joins = reinterpret_cast<const PagedJoin*>(d + at[i].joins);
-    if (i == 2) p->weights = w;
+    if (i == weights_host) p->weights = w;
     else p->works.push_back(w);
   }
   p->slots = reinterpret_cast<const PagedSlots*>(d + at_slots);
