@@ -719,3 +719,14 @@ def test_empty_calls(kvf):
     assert (e.kept == -1).all() and c.length(s) == 0
     b = c.extend([], [], 4)
     assert b.tokens == 0 and c.evict([], 3).seqs == []
+
+
+def test_example_runs():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "paged_cache.py"), "--tokens", "700", "--budget",
+                        "300", "--layers", "2"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "evicted to 300 tokens" in r.stdout and "layer 1:" in r.stdout
