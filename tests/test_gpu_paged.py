@@ -538,6 +538,53 @@ def test_evict(kvf, dtype, D, kind, budget, recent, sinks):
                     assert torch.equal(a[layer, h].nan_to_num(9.0), b[layer, h, want].nan_to_num(9.0))
 
 
+def test_evict_long_sequences(kvf):
+    """More weights than the selection keeps in shared memory (200 KB), and page
+    tables too long to travel with the launch."""
+    page, H, lens = 32, 2, [52000, 70001, 30]
+    budget, recent, sinks = 40000, 100, 4
+    spare = sum(-(-min(n, budget) // page) for n in lens)
+    w = World(kvf, [(n, 0) for n in lens], H, 8, F16, page, seed=6, spare=spare)
+    wt = w.cache.weights
+    wt.copy_(torch.randint(0, 50000, wt.shape, generator=_gen(8), device="cuda").float())
+    old = []
+    for s, n in zip(w.seqs, lens):
+        pages = torch.tensor(w.cache.pages(s), device="cuda")
+        old.append(wt[0, pages].transpose(0, 1).reshape(H, -1)[:, :n].cpu().tolist())
+    e = w.cache.evict(w.seqs, budget, recent, sinks)
+    kept = e.kept[0].cpu()
+    for i, (s, n) in enumerate(zip(w.seqs, lens)):
+        m = min(budget, n)
+        kv = w.cache.gather(s)
+        pages = torch.tensor(w.cache.pages(s), device="cuda")
+        weights = w.cache.weights[0, pages].transpose(0, 1).reshape(H, -1)[:, :m].cpu()
+        for h in range(H):
+            want = _kept(old[i][h], n, budget, recent, sinks)
+            assert kept[i, h, :m].tolist() == want and bool((kept[i, h, m:] == -1).all())
+            at = torch.tensor(want, device="cuda")
+            assert torch.equal(kv.keys_tensor[h], w.k[i][at, h]) and torch.equal(kv.values_tensor[h], w.v[i][at, h])
+            assert weights[h].tolist() == [old[i][h][j] for j in want]
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (F32, 12)])
+@pytest.mark.parametrize("n", [959 * 16, 960 * 16, 960 * 16 + 1, 1920 * 16 - 1, 1920 * 16 + 5])
+def test_gather_of_many_pages(kvf, dtype, D, n):
+    w = World(kvf, [(n, 0)], 2, D, dtype, 16, seed=n % 97)
+    kv = w.cache.gather(w.seqs[0])
+    assert torch.equal(kv.keys_tensor, w.k[0].transpose(0, 1))
+    assert torch.equal(kv.values_tensor, w.v[0].transpose(0, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new,window,sinks", [(1, 0, 0), (1, 100001, 7), (40, 0, 0), (40, 70000, 130)])
+def test_long_sequence(kvf, dtype, new, window, sinks):
+    """150000 slots in 9375 pages, shared out over all multiprocessors, beside a
+    short sequence."""
+    w = World(kvf, [(150000 - new, new), (20, 1)], 1, 64, dtype, 16, seed=new)
+    q = w.step(4, window, sinks)
+    check(w, q, window, sinks, decay=0.0)
+
+
 def test_evict_keeps_the_source(kvf):
     w = World(kvf, [(200, 0), (50, 0)], 2, 64, F16, 16, seed=5, spare=12)
     w.cache.weights.copy_(torch.rand(w.cache.weights.shape, generator=_gen(1), device="cuda"))
