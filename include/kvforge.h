@@ -467,7 +467,9 @@ kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t lay
  * that has new tokens gets weight = decay * weight + sum over the new tokens
  * and the KV head's query heads of the slot's softmax weight (decay 0
  * overwrites). The sums run in a fixed order: results do not change from run
- * to run. Stream-ordered; no host synchronisation. */
+ * to run. Stream-ordered; no host synchronisation. A plan's first call with
+ * decay >= 0 allocates device memory for the weights, which the plan keeps: make
+ * one such call before a stream capture. */
 kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
                                const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
                                float decay, void* out, float* lse, void* stream);

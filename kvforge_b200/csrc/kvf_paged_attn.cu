@@ -133,6 +133,8 @@ __device__ __forceinline__ float half_sum(float v) {
 // Tiles of 64 slots; 64 rows (RT = 4) where there are many, 16 (RT = 1) for
 // single tokens. Bound by the CUDA cores' multiply-adds at 64 rows and by
 // loads at 16; two CTAs (64 rows, head_dim 128: 113 KB each) or three share an SM.
+// 500 f32 tokens on 1548, 32 heads of 128: 641 us (23 TFLOP/s of the products, 739
+// with loads that wait; tiles of 128 rows 654, paired multiply-adds 690).
 template <typename T, int RT, int NU>
 __global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(PagedAttn a, const PagedSeg* __restrict__ segs,
                                                             const int* __restrict__ first, int DP, bool wide,
@@ -298,7 +300,8 @@ __global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(Pag
 // Joins the parts of cut tiles: one warp per row, lanes over the columns. All
 // it needs of the plan is read before it waits for the attention to end, and the
 // first parts' sums and maxima are loaded together; bound by that one latency
-// for short lists, and by reading the parts from L2 for long ones.
+// for short lists, and by reading the parts from L2 for long ones (4.4 us for one
+// sequence of 2048 slots, most of it the wait; 16 for two chunks of 1000 tokens).
 constexpr int kJoinWarps = 4, kJoinAhead = 4;
 template <typename T, int NC>  // NC: columns per lane
 __global__ void __launch_bounds__(32 * kJoinWarps) k_paged_join(PagedAttn a, const PagedJoin* __restrict__ joins,

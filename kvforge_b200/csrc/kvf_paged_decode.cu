@@ -13,7 +13,9 @@
 // the columns of V over all 64 slots. So a segment ends without joining sums
 // across warps, and short sequences cost little more than their loads (with a
 // running maximum and sums of its own for each warp, joined at the end of every
-// segment, a batch of 64 sequences of 0 to 16383 slots took 256 us).
+// segment, a batch of 64 sequences of 0 to 16383 slots took 256 us). That batch,
+// 8 KV heads of 128 in bf16, 632 MB: 104 us, 6.1 TB/s; one sequence of 2048
+// slots, a tile per CTA: 6.2 us, all latency.
 //
 // Slots that no row sees are masked by selection, and their values are
 // replaced by zeros in shared memory, whatever the pages hold. A non-finite
@@ -445,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 // Attention weights from the scores that k_paged_decode wrote: a thread adds
 // four slots' rows in order, 64 threads a (tile, head), the loads of eight rows
-// in flight. Bound by reading the scores, mostly from L2.
+// in flight. Bound by reading the scores, mostly from L2 (10.6 us for 16
+// sequences of 3000 to 16000 slots with 64 query heads; 22 with a slot per thread).
 constexpr int kWeightThreads = 256;
 constexpr int kWeightHeads = kWeightThreads * 4 / kDecodeWeightSlots;
 __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,

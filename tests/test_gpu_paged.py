@@ -421,6 +421,57 @@ def test_other_streams(kvf):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128), (F32, 20)])
+def test_many_sequences(kvf, dtype, dim):
+    """More sequences than multiprocessors by far, most of them shorter than a tile."""
+    rng = np.random.RandomState(dim)
+    lens = [(int(a), int(c)) for a, c in zip(rng.randint(0, 40, 2000), rng.randint(0, 3, 2000))]
+    lens[7], lens[1500] = (900, 30), (0, 40)
+    w = World(kvf, lens, 2, dim, dtype, 16, seed=dim)
+    check(w, w.step(4), decay=0.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_whole_prompt(kvf, dtype):
+    w = World(kvf, [(0, 5001)], 1, 64, dtype, 64, seed=21)
+    check(w, w.step(6, 3000, 5), 3000, 5, decay=0.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_captured_step(kvf, dtype):
+    """A step's calls in a CUDA graph, captured on the stream that the batch was
+    made on, give the bits of the calls themselves, on new inputs too."""
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        w = World(kvf, [(200, 1), (30, 50)], 2, 64, dtype, 16, seed=22)
+        q = w.step(8)
+        n = q.shape[0]
+        k = torch.cat([x[a:] for x, (a, _) in zip(w.k, w.lens)])
+        v = torch.cat([x[a:] for x, (a, _) in zip(w.v, w.lens)])
+
+        def step():
+            w.cache.append(w.batch, k, v)
+            return w.cache.attend(w.batch, q, decay=0.0, return_lse=True)
+
+        step()
+        graph = torch.cuda.CUDAGraph()
+    s.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        out, lse = step()
+    with torch.cuda.stream(s):
+        for seed in (1, 2):
+            for t in (q, k, v):
+                t.copy_(_randn(t.shape, dtype, seed))
+            w.cache.weights.fill_(9.0)
+            graph.replay()
+            got = out.clone(), lse.clone(), w.cache.weights.clone()
+            w.cache.weights.fill_(9.0)
+            want = step() + (w.cache.weights,)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    s.synchronize()
+
+
 def test_layers_are_apart(kvf):
     w = World(kvf, [(40, 3)], 2, 64, F16, 16, layers=3, seed=4)
     q = w.step(4, layer=1)
