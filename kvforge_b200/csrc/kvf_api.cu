@@ -1185,7 +1185,9 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
       add(kPagedChunk, few + 1, most, kChunkRows, kChunkKeys, sms, 4, 2);
     } else {
       add(kPagedGeneric, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1);
-      add(kPagedGeneric, few + 1, most, kGenRows, kGenKeys, 2 * sms, 2, 1);
+      const long long mid = p->dim <= kGenDimLong ? (long long)kGenRows : most;
+      add(kPagedGeneric, few + 1, mid, kGenRows, kGenKeys, 2 * sms, 2, 1);
+      if (mid < most) add(kPagedGeneric, mid + 1, most, kGenRowsLong, kGenKeysLong, sms, 1, 0);
     }
     p->few_rows = true;
     for (size_t i = 0; i < n; ++i)

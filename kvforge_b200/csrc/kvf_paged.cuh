@@ -136,6 +136,8 @@ cudaError_t launch_paged_evict(const int* tables, const int* tables_dev, size_t 
 
 // CUDA-core attention: every type and head_dim up to 256
 constexpr int kGenRows = 64, kGenRowsShort = 16, kGenKeys = 64;
+// tiles for more than kGenRows rows, head_dim up to kGenDimLong
+constexpr int kGenRowsLong = 128, kGenKeysLong = 128, kGenDimLong = 128;
 cudaError_t launch_paged_attn_generic(const PagedAttn& a, const PagedWork& w, cudaStream_t st);
 // joins the partial results of its cut tiles
 cudaError_t launch_paged_join(const PagedAttn& a, const PagedWork& w, cudaStream_t st);

@@ -20,6 +20,9 @@ namespace {
 constexpr int kGenThreads = 256;
 constexpr int kPStride = kGenKeys + 4;  // rows of P, 16-byte aligned, four banks apart
 
+constexpr int kPStrideLong = kGenKeysLong + 16;  // half a set of banks apart: two rows are written at once
+constexpr int kSlabs = 4, kSlabFloats = 32 * 128;
+
 // element (r, c) of a tile of f32 rows in shared memory, rows of DP floats (a
 // multiple of 32): 16-byte groups are permuted by the row so that eight rows
 // at one column lie in different banks
@@ -130,11 +133,9 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // A 16 x 16 arrangement of threads: thread (ty, tx) holds the scores of RT
 // rows and four slots, then those rows' sums of NU groups of four columns.
-// Tiles of 64 slots; 64 rows (RT = 4) where there are many, 16 (RT = 1) for
-// single tokens. Bound by the CUDA cores' multiply-adds at 64 rows and by
+// Tiles of 64 slots; 64 rows (RT = 4), or 16 (RT = 1) for single tokens. Bound
+// by shared-memory loads and the CUDA cores' multiply-adds at 64 rows and by
 // loads at 16; two CTAs (64 rows, head_dim 128: 113 KB each) or three share an SM.
-// 500 f32 tokens on 1548, 32 heads of 128: 641 us (23 TFLOP/s of the products, 739
-// with loads that wait; tiles of 128 rows 654, paired multiply-adds 690).
 template <typename T, int RT, int NU>
 __global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(PagedAttn a, const PagedSeg* __restrict__ segs,
                                                             const int* __restrict__ first, int DP, bool wide,
@@ -292,6 +293,229 @@ __global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(Pag
           const float x = e & 1 ? o[i][u][e >> 1].y : o[i][u][e >> 1].x;
           if (g.part >= 0) a.part_o[((size_t)g.part * BR + r) * D + c] = x;
           else static_cast<T*>(a.out)[at * D + c] = from_float<T>(none ? 0.0f : x * inv);
+        }
+    }
+  }
+}
+
+// The same for more than 64 rows and head dims up to 128, in tiles of 128 rows by
+// 128 slots: a thread's 8 x 8 scores (then 8 rows by 8 columns) take 16 loads of
+// 16 bytes from shared memory per 256 multiply-adds, where the 4 x 4 of the tiles
+// above take 8 per 64. K and V do not fit beside Q and P whole: they pass through
+// a ring of four slabs (128 slots by 32 of the head dim, or 32 slots by the head
+// dim), each loaded while the three before it are worked on, with one barrier per
+// slab. The head dim is filled up to 64 or 128 so that offsets are constants.
+// 500 f32 tokens on 1548, 32 heads of 128: 495 us, 30 TFLOP/s of the products, with
+// 64-row tiles 639; 100 tokens on 1100, 8 heads: 51 against 63 in all; only a single
+// tile is no faster (42 against 40). Bound by issue: two warps a scheduler, an
+// instruction issued in half of the cycles, two thirds of them multiply-adds (loads
+// from shared memory take a third of their pipe). Scalar multiply-adds for P V
+// instead of paired ones: 4 % slower; two steps of the inner loop at once: 3 %.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGenThreads, 1) k_paged_attn_long(PagedAttn a, const PagedSeg* __restrict__ segs,
+                                                                    const int* __restrict__ first, bool wide,
+                                                                    bool wide_q) {
+  constexpr int BR = kGenRowsLong, BK = kGenKeysLong, NU = DP / 64;
+  extern __shared__ float4 sm4[];
+  float* Q = reinterpret_cast<float*>(sm4);  // [BR][DP]
+  float* P = Q + BR * DP;                    // [BR][kPStrideLong]
+  float* ring = P + BR * kPStrideLong;       // kSlabs of kSlabFloats
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;  // rows ty + 16 i, slots tx + 16 u
+  const int D = a.c.dim, Hq = a.c.heads * a.group;
+  const int k_slabs = (D + 31) / 32, per = k_slabs + BK / 32;
+  const int s1 = __ldg(first + blockIdx.x + 1);
+  for (int si = __ldg(first + blockIdx.x); si < s1; ++si) {
+    const PagedSeg g = segs[si];
+    const int n = __ldg(a.s.kv_len + g.seq), q0 = __ldg(a.s.q_start + g.seq);
+    const int nq = __ldg(a.s.q_start + g.seq + 1) - q0, rows = min(BR, nq * a.group - g.row0);
+    const int* table = a.s.table + (size_t)g.seq * a.s.stride;
+    const PagedSpan span = paged_span(g.row0, BR, a.group, n, nq, a.window, a.sinks, BK);
+    __syncthreads();  // the previous segment's tiles are read
+    fill_tile<T>(Q, BR, DP, D, wide_q, [&](int r) -> const T* {
+      if (r >= rows) return nullptr;
+      const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+      return static_cast<const T*>(a.q) + (size_t)(q0 + t) * a.q_token + (size_t)hq * a.q_head;
+    });
+    float m[8], l[8];
+    float2 o[8][NU][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) o[i][u][0] = o[i][u][1] = make_float2(0.0f, 0.0f);
+    }
+    const int pa = n - nq + g.row0 / a.group, pb = n - nq + (g.row0 + rows - 1) / a.group;
+    auto slot0 = [&](int it) { return (it < span.nsink ? it : span.first + it - span.nsink) * BK; };
+    // the next slab of the segment into its place (nothing behind the last one,
+    // but a group all the same, so that every step waits for the same number)
+    int load_it = g.it0, load_x = 0, load_at = 0;
+    auto load = [&] {
+      if (load_it < g.it1) {
+        const int j0 = slot0(load_it);
+        // slots that no row of the tile sees are zeros here
+        auto row = [&](const void* pool, int j) -> const T* {
+          if (j > pb || (a.window && j <= pa - a.window && j >= a.sinks)) return nullptr;
+          return static_cast<const T*>(pool) + paged_row(table, a.c, g.head, j);
+        };
+        float* to = ring + load_at * kSlabFloats;
+        if (load_x < k_slabs) {
+          const int d0 = 32 * load_x;
+          fill_tile<T>(to, BK, 32, D - d0, wide, [&](int r) -> const T* {
+            const T* p = row(a.c.keys, j0 + r);
+            return p ? p + d0 : nullptr;
+          });
+        } else {
+          const int r0 = j0 + 32 * (load_x - k_slabs);
+          fill_tile<T>(to, 32, DP, D, wide, [&](int r) { return row(a.c.values, r0 + r); });
+        }
+        if (++load_x == per) {
+          load_x = 0;
+          ++load_it;
+        }
+      } else {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      load_at = (load_at + 1) % kSlabs;
+    };
+    int at = 0;
+    auto next = [&] {  // the next slab to work on; the one before it makes room
+      filled<kSlabs - 2>();
+      __syncthreads();
+      load();
+      const float* p = ring + at * kSlabFloats;
+      at = (at + 1) % kSlabs;
+      return p;
+    };
+#pragma unroll 1
+    for (int k = 0; k < kSlabs - 1; ++k) load();
+    for (int it = g.it0; it < g.it1; ++it) {
+      const int j0 = slot0(it);
+      float s[8][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s[i][u] = 0.0f;
+#pragma unroll 1
+      for (int x = 0; x < k_slabs; ++x) {
+        const float* kp = next() + tx * 32;
+        const float* qp = Q + ty * DP + 32 * x;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          // (rows 16 apart have the same permutation of their pieces)
+          const int qc = (c ^ (ty & 7)) << 2, kc = (c ^ (tx & 7)) << 2;
+          float4 q[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) q[i] = *reinterpret_cast<const float4*>(qp + 16 * i * DP + qc);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const float4 k = *reinterpret_cast<const float4*>(kp + 16 * u * 32 + kc);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              s[i][u] = fmaf(q[i].x, k.x, s[i][u]);
+              s[i][u] = fmaf(q[i].y, k.y, s[i][u]);
+              s[i][u] = fmaf(q[i].z, k.z, s[i][u]);
+              s[i][u] = fmaf(q[i].w, k.w, s[i][u]);
+            }
+          }
+        }
+      }
+      const bool whole = j0 + BK - 1 <= pa && (!a.window || j0 > pb - a.window || j0 + BK <= a.sinks);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        unsigned see = 0xffu;  // which of its eight slots the row sees
+        if (!whole) {
+          const int pos = n - nq + (g.row0 + ty + 16 * i) / a.group;
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (!paged_sees(pos, j0 + tx + 16 * u, a.window, a.sinks)) see ^= 1u << u;
+        }
+        float mx = m[i];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          s[i][u] = (see >> u & 1) ? s[i][u] * a.scale2 : -INFINITY;
+          mx = fmaxf(mx, s[i][u]);
+        }
+        mx = half_max(mx);
+        const float mu = mx == -INFINITY ? 0.0f : mx;  // nothing seen yet: all terms are 0
+        const float f = exp2f(m[i] - mu);
+        m[i] = mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float p = exp2f(s[i][u] - mu);
+          sum += p;
+          // a slot that the row does not see is marked, see above
+          P[(ty + 16 * i) * kPStrideLong + tx + 16 * u] = (see >> u & 1) ? p : -1.0f;
+        }
+        l[i] = l[i] * f + half_sum(sum);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            o[i][u][e].x *= f;
+            o[i][u][e].y *= f;
+          }
+      }
+      __syncwarp();  // a half-warp reads its own rows of P only
+      auto accumulate = [&](const float* v_slab, const float* pp, auto masked) {
+#pragma unroll 1
+        for (int k4 = 0; k4 < 32; k4 += 4) {
+          float4 p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = *reinterpret_cast<const float4*>(pp + 16 * i * kPStrideLong + k4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+              const float4 v = *reinterpret_cast<const float4*>(v_slab + tile_at(k4 + kk, tx + 16 * u, DP));
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float pk = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
+                if (decltype(masked)::value && pk < 0.0f) continue;
+                const float2 p2 = make_float2(pk, pk);
+                o[i][u][0] = ffma2(p2, make_float2(v.x, v.y), o[i][u][0]);
+                o[i][u][1] = ffma2(p2, make_float2(v.z, v.w), o[i][u][1]);
+              }
+            }
+        }
+      };
+#pragma unroll 1
+      for (int x = 0; x < BK / 32; ++x) {
+        const float* v = next();
+        if (j0 + 32 * x > pb) continue;
+        const float* pp = P + ty * kPStrideLong + 32 * x;
+        if (whole) accumulate(v, pp, std::false_type{});
+        else accumulate(v, pp, std::true_type{});
+      }
+    }
+    filled<0>();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = ty + 16 * i;
+      if (r >= rows) continue;
+      const int t = (g.row0 + r) / a.group, hq = g.head * a.group + (g.row0 + r) % a.group;
+      const size_t to = (size_t)(q0 + t) * Hq + hq;
+      const bool none = l[i] == 0.0f;
+      const float inv = none ? 0.0f : 1.0f / l[i];
+      if (tx == 0) {
+        if (g.part >= 0) {
+          float* ml = a.part_ml + ((size_t)g.part * BR + r) * 2;
+          ml[0] = m[i];
+          ml[1] = l[i];
+        } else if (a.lse) {
+          a.lse[to] = none ? -INFINITY : (m[i] + log2f(l[i])) * (float)M_LN2;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 4 * (tx + 16 * u) + e;
+          if (c >= D) continue;
+          const float x = e & 1 ? o[i][u][e >> 1].y : o[i][u][e >> 1].x;
+          if (g.part >= 0) a.part_o[((size_t)g.part * BR + r) * D + c] = x;
+          else static_cast<T*>(a.out)[to * D + c] = from_float<T>(none ? 0.0f : x * inv);
         }
     }
   }
@@ -458,8 +682,22 @@ cudaError_t attn_launch(const PagedAttn& a, const PagedWork& w, cudaStream_t st)
   return cudaGetLastError();
 }
 
+template <typename T, int DP>
+cudaError_t attn_long_launch(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  constexpr size_t smem = ((size_t)kGenRowsLong * (DP + kPStrideLong) + kSlabs * kSlabFloats) * sizeof(float);
+  auto kern = k_paged_attn_long<T, DP>;
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<w.ctas, kGenThreads, smem, st>>>(a, w.segs, w.first, wide_rows<T>(a), wide_query<T>(a));
+  note_launches(1);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t attn_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
+  if (w.row_tile == kGenRowsLong)
+    return a.c.dim <= 64 ? attn_long_launch<T, 64>(a, w, st) : attn_long_launch<T, kGenDimLong>(a, w, st);
   const int nu = (a.c.dim + 63) / 64;
   if (w.row_tile == kGenRows)
     return nu == 1 ? attn_launch<T, 4, 1>(a, w, st) : nu == 2 ? attn_launch<T, 4, 2>(a, w, st)
