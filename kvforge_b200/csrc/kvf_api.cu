@@ -1185,7 +1185,19 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
       add(kPagedChunk, few + 1, most, kChunkRows, kChunkKeys, sms, 4, 2);
     } else {
       add(kPagedGeneric, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1);
-      const long long mid = p->dim <= kGenDimLong ? (long long)kGenRows : most;
+      // Sequences of more than kGenRows rows: a tile of 128 x 128 takes an SM 2.75
+      // times as long as one of 64 x 64 (35 and 12.7 us at head_dim 128), and there
+      // are four of those to one, or fewer in narrow windows: eight chunks of 392
+      // tokens, 128 query heads, window of 2: 1026 us with large tiles, 830 with
+      // small ones; of 100: 1657 and 1641; of 1000: 4230 and 5300
+      long long mid = most;
+      if (p->dim <= kGenDimLong) {
+        auto tiles = [&](int row_tile, int key_tile) {
+          return paged_tiles(q_lens, kv_lens, n, heads, group, p->window, p->sinks, kGenRows + 1, most, row_tile,
+                             key_tile);
+        };
+        if (11 * tiles(kGenRowsLong, kGenKeysLong) <= 4 * tiles(kGenRows, kGenKeys)) mid = kGenRows;
+      }
       add(kPagedGeneric, few + 1, mid, kGenRows, kGenKeys, 2 * sms, 2, 1);
       if (mid < most) add(kPagedGeneric, mid + 1, most, kGenRowsLong, kGenKeysLong, sms, 1, 0);
     }

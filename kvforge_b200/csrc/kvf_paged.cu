@@ -71,6 +71,18 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
   }
 }
 
+long long paged_tiles(const int* q_lens, const int* kv_lens, size_t n, int heads, int group, int window, int sinks,
+                      long long lo, long long hi, int row_tile, int key_tile) {
+  long long tiles = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const long long rows = (long long)q_lens[i] * group;
+    if (rows < lo || rows > hi) continue;
+    for (int r = 0; r < rows; r += row_tile)
+      tiles += (long long)heads * paged_span(r, row_tile, group, kv_lens[i], q_lens[i], window, sinks, key_tile).count;
+  }
+  return tiles;
+}
+
 namespace {
 
 constexpr int kCopyThreads = 256;

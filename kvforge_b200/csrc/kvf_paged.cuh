@@ -118,6 +118,10 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
                  long long lo, long long hi, int row_tile, int key_tile, int slots, int least, int fixed,
                  PagedWorkHost* out);
 
+// Iterations of those row tiles.
+long long paged_tiles(const int* q_lens, const int* kv_lens, size_t n, int heads, int group, int window, int sinks,
+                      long long lo, long long hi, int row_tile, int key_tile);
+
 // ---- launchers ---------------------------------------------------------------
 // place [tokens]: page * 128 + row of every token, -1 for none
 cudaError_t launch_paged_append(const long long* place, const PagedLayer& c, size_t tokens, const void* k, size_t kt,
