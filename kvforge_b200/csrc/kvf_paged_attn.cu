@@ -587,7 +587,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_paged_join(PagedAttn a, con
 
 // Attention weight of 64 slots of one (sequence, head): the column sums of
 // the softmax over all rows that may see them, each row's sum known from lse.
-// A CTA owns its slots and adds its rows in a fixed order: no atomics.
+// A CTA owns its slots and adds its rows in a fixed order: no atomics. Rows come
+// in tiles of 16 RT: 16 where no sequence has more, 128 otherwise (f32, 500 tokens
+// on 1548 with 32 heads of 128: 336 us, 356 in tiles of 64 rows; of 256: 686 and
+// 898). Bound as the attention itself: shared-memory loads and multiply-adds.
 template <typename T, int RT>
 __global__ void __launch_bounds__(kGenThreads) k_paged_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,
                                                                float decay, int DP, bool wide, bool wide_q) {
@@ -731,7 +734,7 @@ template <typename T>
 cudaError_t weights_typed(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, bool few_rows, float decay,
                           cudaStream_t st) {
   return few_rows ? weights_launch<T, 1>(a, tiles, ntiles, decay, st)
-                  : weights_launch<T, 4>(a, tiles, ntiles, decay, st);
+                  : weights_launch<T, 8>(a, tiles, ntiles, decay, st);
 }
 
 }  // namespace
