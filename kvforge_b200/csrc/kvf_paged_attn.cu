@@ -267,6 +267,9 @@ __global__ void __launch_bounds__(kGenThreads, NU <= 2 ? 2 : 1) k_paged_attn(Pag
         fill(V, a.c.values, it + 1);
       }
     }
+    // copies to one place are in no order: those of a segment without tiles (its
+    // rows) have to land before the next segment's start
+    filled<0>();
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int r = ty * RT + i;
@@ -643,6 +646,7 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_weights(PagedAttn a, cons
         if (paged_sees(pos, j0 + tx + 16 * u, a.window, a.sinks)) w[u] += exp2f(fmaf(s[i][u], a.scale2, -z));
     }
   }
+  filled<0>();  // K, where no row sees the slots
 #pragma unroll
   for (int u = 0; u < 4; ++u) sums[ty][tx + 16 * u] = w[u];
   __syncthreads();

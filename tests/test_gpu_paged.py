@@ -828,3 +828,29 @@ def test_example_runs():
                         "300", "--layers", "2"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "evicted to 300 tokens" in r.stdout and "layer 1:" in r.stdout
+
+
+# ---- rows, batches and calls out of the ordinary ------------------------------------------
+@pytest.mark.parametrize("D", [20, 64, 100, 128, 200, 256])
+@pytest.mark.parametrize("queries", [4, 16, 100, 900])
+def test_rows_of_a_tile_without_slots_then_others(kvf, D, queries):
+    """f32, whose rows are copied asynchronously: many tiles of rows that see
+    nothing, each followed by tiles that see slots, in one CTA's share."""
+    H, G, n = 2, 4, 24
+    lens = [(7, 0), (90, 3)] * n
+    w = World(kvf, lens, H, D, F32, 16, seed=D)
+    w.step(H * G)
+    counts = [queries, 3] * n
+    b = w.cache.batch(w.seqs, counts, H * G)
+    q = _randn((sum(counts), H * G, D), F32, 3)
+    first = w.cache.attend(b, q, return_lse=True, decay=0.0)
+    at = 0
+    for i, c in enumerate(counts):
+        if i < 4 or i >= 2 * n - 4:
+            o, z, _, to, tz, _ = reference(w.k[i], w.v[i], q[at:at + c], D ** -0.5, 0, 0, F32)
+            close(first[0][at:at + c], o, to, f"out of sequence {i}")
+            close(first[1][at:at + c], z, tz, f"lse of sequence {i}")
+        at += c
+    for _ in range(5):
+        for x, y in zip(first, w.cache.attend(b, q, return_lse=True, decay=0.0)):
+            assert torch.equal(x, y)
