@@ -340,6 +340,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
           if (bad) sh.bad[si & 1] = 1;
+          // the stage's next tile is written by tensor-map loads: behind these stores
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         consumer_sync();  // the maxima are there
         if (sh.stop) {

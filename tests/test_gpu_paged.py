@@ -854,3 +854,19 @@ def test_rows_of_a_tile_without_slots_then_others(kvf, D, queries):
     for _ in range(5):
         for x, y in zip(first, w.cache.attend(b, q, return_lse=True, decay=0.0)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("c,window,sinks", [(1, 0, 0), (4, 0, 0), (2, 40, 3), (1, 65, 70)])
+def test_tiles_put_right_and_loaded_over(kvf, dtype, D, c, window, sinks):
+    """Many short sequences whose tiles all have masked slots: values that are
+    replaced in shared memory (the pages around them hold NaN) and the next tiles
+    that arrive in the same place, without a trace of one in the other."""
+    rng = np.random.RandomState(D + c)
+    lens = [(int(a), c) for a in rng.randint(0, 140, 160)]
+    w = World(kvf, lens, 4, D, dtype, 16, seed=c + window)
+    q = w.step(16, window, sinks)
+    first = check(w, q, window, sinks)
+    for _ in range(10):
+        for x, y in zip(first, w.cache.attend(w.batch, q, return_lse=True)):
+            assert torch.equal(x, y)
