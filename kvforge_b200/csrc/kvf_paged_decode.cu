@@ -451,10 +451,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 // four slots' rows in order, 64 threads a (tile, head), the loads of eight rows
 // in flight. Bound by reading the scores, mostly from L2 (10.6 us for 16
 // sequences of 3000 to 16000 slots with 64 query heads; 22 with a slot per thread).
+// The scores may still be written while this kernel starts: ordinary loads behind
+// the wait, never the read-only path.
 constexpr int kWeightThreads = 256;
 constexpr int kWeightHeads = kWeightThreads * 4 / kDecodeWeightSlots;
 __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAttn a, const PagedSlots* __restrict__ tiles,
-                                                                         const float* __restrict__ scores,
+                                                                         const float* scores,
                                                                          const long long* __restrict__ score_at,
                                                                          float decay) {
   __shared__ float lse2[kWeightHeads][kRows];
@@ -489,7 +491,7 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAt
       float4 x[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r)
-        if (r0 + r < rows) x[r] = __ldg(reinterpret_cast<const float4*>(sc + (r0 + r) * sc_row));
+        if (r0 + r < rows) x[r] = *reinterpret_cast<const float4*>(sc + (r0 + r) * sc_row);
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         if (r0 + r >= rows) continue;

@@ -366,11 +366,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
-// weight = decay * weight + the parts of its slot
+// weight = decay * weight + the parts of its slot (written by the kernel before,
+// whose end this one overlaps: ordinary loads behind the wait)
 __global__ void __launch_bounds__(kWeightSlots) k_paged_chunk_weights_join(PagedAttn a,
                                                                            const PagedJoin* __restrict__ joins,
-                                                                           const float* __restrict__ part_w,
-                                                                           float decay) {
+                                                                           const float* part_w, float decay) {
   const PagedJoin g = joins[blockIdx.x];
   const int j = g.row0 + threadIdx.x;
   const bool there = j < __ldg(a.s.kv_len + g.seq);
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kWeightSlots) k_paged_chunk_weights_join(Paged
   if (!there) return;
   float t = 0.0f;
 #pragma unroll 4
-  for (int p = 0; p < 2 * g.parts; ++p) t += __ldg(part_w + ((size_t)2 * g.part0 + p) * kWeightSlots + threadIdx.x);
+  for (int p = 0; p < 2 * g.parts; ++p) t += part_w[((size_t)2 * g.part0 + p) * kWeightSlots + threadIdx.x];
   const int page = __ldg(a.s.table + (size_t)g.seq * a.s.stride + (j >> a.c.page_shift));
   float* p = a.c.weights + (((size_t)page * a.c.heads + g.head) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
   *p = decay == 0.0f ? t : fmaf(decay, *p, t);

@@ -870,3 +870,24 @@ def test_tiles_put_right_and_loaded_over(kvf, dtype, D, c, window, sinks):
     for _ in range(10):
         for x, y in zip(first, w.cache.attend(w.batch, q, return_lse=True)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", [1, 4, 6, 10, 14])
+def test_weights_of_queries_in_turn(kvf, dtype, case):
+    """Calls of one batch share scores and parts of sums: each call's weights are
+    its own queries', right behind those of others."""
+    lens, H, G, D, page = SHAPES[case]
+    w = World(kvf, lens, H, D, dtype, page, seed=case)
+    w.cache.weights.zero_()
+    qs = [w.step(H * G)] + [_randn((w.batch.tokens, H * G, D), dtype, 50 + i) for i in range(2)]
+    want = []
+    for q in qs:
+        check(w, q, decay=0.0)
+        want.append(w.cache.weights.clone())
+    got = []
+    for i in range(30):
+        w.cache.attend(w.batch, qs[i % 3], decay=0.0)
+        got.append(w.cache.weights.clone())
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 3]), i
