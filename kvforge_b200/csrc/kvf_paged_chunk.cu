@@ -65,9 +65,11 @@ constexpr int stages() { return DP == 128 ? 5 : 10; }
 template <int DP>
 struct Shared {
   uint64_t bars[3 * stages<DP>() + 6 * kTiles];
-  // segment that last had non-finite values in tiles not seen whole, by the
-  // segment's index mod 8 (loads run less than three segments ahead)
-  int bad[8];
+  // segment that last had non-finite values in tiles not seen whole: places 0 and
+  // 1 in turn for segments of two row tiles, 2 and 3 for those of one. (The second
+  // row tile may still look a segment up while the first is past any number of
+  // single ones, but the first begins a third of two tiles only behind its turn.)
+  int bad[4];
   uint32_t tmem;
   int abort;
 };
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(turn + 8 * i, 4);
     }
     sh.abort = 0;
-    for (int i = 0; i < 8; ++i) sh.bad[i] = -1;
+    for (int i = 0; i < 4; ++i) sh.bad[i] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -317,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int cnt_s = 0, cnt_o = 0;
     uint32_t turns = 0;
     int ring0 = 0;  // tiles of K and V before this segment
+    uint32_t bad_at = 0;  // bit 0: the place of the next segment of two row tiles, bit 1: of one
     for (int si = seg0; si < seg1; ++si) {
       const Seg s(a, segs[si]);
       const int count = s.g.it1 - s.g.it0;
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (bad) sh.bad[si & 7] = si;
+          if (bad) sh.bad[two ? bad_at & 1 : 2 + (bad_at >> 1)] = si;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor core reads what was written
           __syncwarp();
           if (lane == 0) mbar_arrive(fixed + 8 * st);
@@ -494,7 +497,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_after();
       }
       if (gave_up) break;
-      const bool bad = count > 0 && sh.bad[si & 7] == si;
+      bool bad = false;
+      if (count > 0) {
+        bad = sh.bad[two ? bad_at & 1 : 2 + (bad_at >> 1)] == si;
+        bad_at ^= two ? 1u : 2u;
+      }
       const bool none = l == 0.0f;
       const float inv = none ? 0.0f : 1.0f / l;
       const size_t at = (size_t)(s.q0 + tok) * (a.c.heads * a.group) + hq;

@@ -891,3 +891,33 @@ def test_weights_of_queries_in_turn(kvf, dtype, case):
         got.append(w.cache.weights.clone())
     for i, x in enumerate(got):
         assert torch.equal(x, want[i % 3]), i
+
+
+@pytest.mark.parametrize("dtype,D", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("singles", [1, 9, 30])
+def test_infinite_values_of_long_and_short_rows_in_turn(kvf, dtype, D, singles):
+    """Shares of many segments, of one and of two row tiles: an infinite value
+    reaches its own sequence's rows that see it, and no others. All other values
+    are 1, so that an output is 1 to within the numerators' and its own rounding
+    (u each) and the f32 sums' (less than u)."""
+    H, G = 8, 4
+    lens = ([(10, 45)] + [(5, 6 + i % 20) for i in range(singles)]) * (200 // (singles + 1))
+    w = World(kvf, lens, H, D, dtype, 16, seed=singles)
+    rng = np.random.RandomState(singles)
+    want, at = [], 0
+    for i, (a, c) in enumerate(lens):
+        w.v[i].fill_(1.0)
+        inf = torch.zeros((c, H, D), dtype=torch.bool, device="cuda")
+        if i % 3 != 1:
+            j, h, col = int(rng.randint(a, a + c)), int(rng.randint(H)), int(rng.randint(D))
+            w.v[i][j, h, col] = math.inf
+            inf[j - a:, h, col] = True  # the rows from its own token on
+        want.append(inf.repeat_interleave(G, 1))
+    old = w.cache.batch(w.seqs, [a for a, _ in lens])
+    w.cache.append(old, torch.cat([k[:a] for k, (a, _) in zip(w.k, lens)]),
+                   torch.cat([v[:a] for v, (a, _) in zip(w.v, lens)]))
+    q, want = w.step(H * G), torch.cat(want)
+    for _ in range(5):
+        out = w.cache.attend(w.batch, q)
+        assert torch.equal(torch.isinf(out), want)
+        assert (out[~want].double() - 1.0).abs().max() <= 3 * UNIT[dtype]
