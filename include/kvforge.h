@@ -433,7 +433,8 @@ typedef struct {
  * any stream, by one host thread at a time: its calls run one after another on
  * the GPU, also when they are issued on different streams. kvf_paged_plan_free
  * returns its memory after the last call issued with it on every stream;
- * `stream` and the context must outlive it. */
+ * `stream` and the context must outlive it. No plan is made inside a stream
+ * capture (KVF_ERR_PIPELINE); calls of one may be captured on `stream`. */
 kvf_status kvf_paged_plan_create(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs,
                                  const int32_t* query_lens_host, const int32_t* kv_lens_host,
                                  const int32_t* page_table_host, size_t table_stride, size_t query_heads,
@@ -469,7 +470,8 @@ kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t lay
  * overwrites). The sums run in a fixed order: results do not change from run
  * to run. Stream-ordered; no host synchronisation. A plan's first call with
  * decay >= 0 allocates device memory for the weights, which the plan keeps: make
- * one such call before a stream capture. */
+ * one such call, with or without lse, before a stream capture of others
+ * (KVF_ERR_PIPELINE inside one). */
 kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
                                const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
                                float decay, void* out, float* lse, void* stream);
@@ -483,7 +485,9 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
  * sources' or named twice; the sources stay as they are. A sequence of at most
  * `budget` slots keeps them all. kept (device) [num_layers, num_seqs, num_heads,
  * budget] i32: the slots, -1 behind the last. The host arrays are read before
- * the call returns. KVF_ERR_INVALID_CONFIG when sinks + recent > budget. */
+ * the call returns. KVF_ERR_INVALID_CONFIG when sinks + recent > budget;
+ * KVF_ERR_PIPELINE inside a stream capture when the tables are too long to be
+ * kernel parameters (960 words in all). */
 kvf_status kvf_paged_evict(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t num_seqs, const int32_t* kv_lens_host,
                            const int32_t* page_table_host, size_t table_stride, size_t budget, size_t recent,
                            size_t sinks, const int32_t* new_table_host, size_t new_table_stride, int32_t* kept,

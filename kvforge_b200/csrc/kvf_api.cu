@@ -1084,8 +1084,20 @@ struct BlockImage {
   }
 };
 
+// Memory that outlives the call, and buffers that the next call reuses, must not
+// become part of a graph: a graph's memory is only there while it runs, and a
+// replayed copy would read what the buffer holds then.
+kvf_status not_capturing(cudaStream_t st, const char* what) {
+  cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+  KVF_CUDA(cudaStreamIsCapturing(st, &c));
+  if (c != cudaStreamCaptureStatusNone)
+    return fail(KVF_ERR_PIPELINE, std::string(what) + " inside a stream capture is not supported");
+  return KVF_OK;
+}
+
 // `bytes` host bytes to the device, through a pinned buffer, without waiting
 kvf_status upload(kvf_ctx* ctx, void* dst, const void* src, size_t bytes, cudaStream_t st) {
+  KVF_TRY(not_capturing(st, "a copy of page tables to the device"));
   kvf_ctx::Pinned pin;
   KVF_CUDA(ctx->pinned(bytes, &pin));
   std::memcpy(pin.p, src, bytes);
@@ -1116,9 +1128,10 @@ kvf_status plan_enter(const kvf_paged_plan* p, cudaStream_t st) {
 
 // the plan's workspace of `n` floats, allocated on first use
 kvf_status plan_floats(const kvf_paged_plan* p, float** at, size_t n, cudaStream_t st) {
-  if (!*at)
-    KVF_CUDA(cudaMallocFromPoolAsync(reinterpret_cast<void**>(at), std::max<size_t>(n, 1) * sizeof(float),
-                                     p->ctx->pool, st));
+  if (*at) return KVF_OK;
+  KVF_TRY(not_capturing(st, "a plan's first call with decay >= 0"));
+  KVF_CUDA(cudaMallocFromPoolAsync(reinterpret_cast<void**>(at), std::max<size_t>(n, 1) * sizeof(float),
+                                   p->ctx->pool, st));
   return KVF_OK;
 }
 
@@ -2468,6 +2481,7 @@ kvf_status kvf_paged_plan_create(kvf_ctx* ctx, const kvf_paged_pool* pool, size_
   if (query_heads > 65535) return fail(KVF_ERR_SHAPE_MISMATCH, "query_heads > 65535 is not supported");
   if (window < 0 || sinks < 0) return fail(KVF_ERR_INVALID_CONFIG, "window and sinks must not be negative");
   DeviceGuard g(ctx->device);
+  KVF_TRY(not_capturing(S(stream), "making a plan"));
   kvf_paged_plan* p = nullptr;
   kvf_status s;
   try {  // no exception leaves the C ABI
@@ -2579,7 +2593,8 @@ kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const k
   KVF_TRY(plan_enter(plan, st));
   const bool track = decay >= 0.0f;
   if (track) {
-    if (!lse) KVF_TRY(plan_floats(plan, &plan->lse, plan->tokens * plan->heads * plan->group, st));
+    // (also where this call's caller takes the lse: a later one may not)
+    KVF_TRY(plan_floats(plan, &plan->lse, plan->tokens * plan->heads * plan->group, st));
     if (plan->scores_n) KVF_TRY(plan_floats(plan, &plan->scores, plan->scores_n, st));
     if (plan->weights.parts)
       KVF_TRY(plan_floats(plan, &plan->part_w, (size_t)2 * plan->weights.parts * kWeightSlots, st));

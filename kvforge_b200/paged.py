@@ -89,7 +89,9 @@ class PagedKVCache:
     Calls are stream-ordered on the current stream; a call on another stream
     than the one before first waits for that one. One host thread at a time.
     append and attend can be captured in a CUDA graph on the stream that the
-    batch was made on, after one such call there; the batch must outlive the graph."""
+    batch was made on, attend with `decay` after one call of that batch with a
+    `decay` (its workspace is not made inside a capture; nor is a batch). The
+    batch must outlive the graph."""
 
     def __init__(self, num_pages: int, num_heads: int, head_dim: int, page_size: int = 64, num_layers: int = 1,
                  dtype: torch.dtype = torch.float16, device=None):

@@ -921,3 +921,60 @@ def test_infinite_values_of_long_and_short_rows_in_turn(kvf, dtype, D, singles):
         out = w.cache.attend(w.batch, q)
         assert torch.equal(torch.isinf(out), want)
         assert (out[~want].double() - 1.0).abs().max() <= 3 * UNIT[dtype]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_captured_step_after_a_call_that_took_the_lse(kvf, dtype):
+    """The workspace of the first call with decay serves every later one: a graph
+    of calls without lse, replayed between calls of their own."""
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        w = World(kvf, [(200, 1), (30, 50)], 2, 64, dtype, 16, seed=22)
+        q = w.step(8)
+        w.cache.weights.fill_(0.0)
+        w.cache.attend(w.batch, q, decay=0.0, return_lse=True)
+        want_w = w.cache.weights.clone()
+        graph = torch.cuda.CUDAGraph()
+    s.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        out = w.cache.attend(w.batch, q, decay=0.0)
+    with torch.cuda.stream(s):
+        want = w.cache.attend(w.batch, q, decay=0.0)
+        live = torch.tensor(sum((w.cache.pages(x) for x in w.seqs), []), device="cuda")
+        for _ in range(3):
+            w.cache.weights.fill_(9.0)
+            out.fill_(9.0)
+            graph.replay()
+            a, b = w.cache.weights[:, live], want_w[:, live]
+            assert torch.equal(out, want) and torch.equal(w.cache.attend(w.batch, q, decay=0.0), want)
+            assert torch.equal(a[a != 9.0], b[a != 9.0]) and (a != 9.0).sum() == 2 * 281
+    s.synchronize()
+    del graph
+
+
+def test_what_a_capture_refuses(kvf):
+    """A batch, the first call with decay, and an eviction with long tables keep
+    memory or read buffers that a graph must not hold: errors, lengths as before."""
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        w = World(kvf, [(200, 1), (30, 50), (20000, 0)], 2, 64, F16, 16, seed=23, spare=20)
+        q = w.step(8)
+        want = w.cache.attend(w.batch, q)
+        graph = torch.cuda.CUDAGraph()
+        lengths, free = [w.cache.length(x) for x in w.seqs], w.cache.free_pages
+    s.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        for call in (lambda: w.cache.extend(w.seqs, [1, 1, 1], 8), lambda: w.cache.batch(w.seqs, [1, 1, 1], 8),
+                     lambda: w.cache.attend(w.batch, q, decay=1.0),
+                     lambda: w.cache.attend(w.batch, q, decay=1.0, return_lse=True),
+                     lambda: w.cache.evict(w.seqs[2], 100)):
+            with pytest.raises(kvf.KvForgeError, match="capture"):
+                call()
+        out = w.cache.attend(w.batch, q)
+    assert [w.cache.length(x) for x in w.seqs] == lengths and w.cache.free_pages <= free
+    with torch.cuda.stream(s):
+        graph.replay()
+        assert torch.equal(out, want)
+        check(w, q, decay=0.0)
+    s.synchronize()
+    del graph
