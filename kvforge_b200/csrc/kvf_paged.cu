@@ -20,10 +20,12 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
   auto span = [&](size_t i, int row0) {
     return paged_span(row0, row_tile, group, kv_lens[i], q_lens[i], window, sinks, key_tile).count;
   };
+  // a tile that sees no slot is a segment all the same: its rows are written
+  auto price = [&](int iterations) { return std::max(iterations, 1) + fixed; };
   long long cost = 0;
   for (size_t i = 0; i < n; ++i)
     if (chosen(i))
-      for (int r = 0; r < q_lens[i] * group; r += row_tile) cost += (long long)heads * (span(i, r) + fixed);
+      for (int r = 0; r < q_lens[i] * group; r += row_tile) cost += (long long)heads * price(span(i, r));
   if (!cost) return;
   long long quota = std::max<long long>((cost + slots - 1) / slots, least + fixed);
   // a CTA that closes early (what is left of its quota is too short to cut a
@@ -53,7 +55,7 @@ void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int
             if (count - it - take < least) take = count - it;  // no sliver behind the cut
             out->segs.push_back({(int)i, h, r, it, it + take, -1});
             it += take;
-            left -= take + fixed;
+            left -= price(take);
             if (left <= fixed) close();
           } while (it < count);
           const int parts = (int)(out->segs.size() - seg0);

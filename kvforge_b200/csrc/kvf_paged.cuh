@@ -111,9 +111,9 @@ struct PagedWorkHost {
   std::vector<PagedJoin> joins;
 };
 // Splits the row tiles of the sequences with lo <= rows <= hi (rows = new
-// tokens * group) over at most `slots` CTAs of equal cost (iterations, plus
-// `fixed` for every segment); no segment but a tile's last is shorter than
-// `least` iterations.
+// tokens * group) over at most `slots` CTAs of equal cost (iterations, at least
+// one, plus `fixed` for every segment); no segment but a tile's last is shorter
+// than `least` iterations. A tile without iterations is one segment.
 void paged_split(const int* q_lens, const int* kv_lens, size_t n, int heads, int group, int window, int sinks,
                  long long lo, long long hi, int row_tile, int key_tile, int slots, int least, int fixed,
                  PagedWorkHost* out);

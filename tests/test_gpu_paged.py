@@ -978,3 +978,36 @@ def test_what_a_capture_refuses(kvf):
         check(w, q, decay=0.0)
     s.synchronize()
     del graph
+
+
+def _attend_into(w, b, q, value):
+    """kvf_paged_attention on outputs that hold `value` before the call."""
+    from kvforge_b200 import _lib as L
+    out, lse = torch.full_like(q, value), torch.full(q.shape[:2], value, dtype=F32, device="cuda")
+    L.check(L.lib().kvf_paged_attention(
+        L.context(0), b._h, C.byref(w.cache._pool), 0, q.data_ptr(), q.stride(0), q.stride(1),
+        w.D ** -0.5, -1.0, out.data_ptr(), lse.data_ptr(),
+        torch.cuda.current_stream().cuda_stream))
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (F32, 128), (F32, 200), (F16, 20), (BF16, 36), (F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("queries", [3, 70, 300])
+@pytest.mark.parametrize("beside", [None, (9, 1), (400, 90)])
+def test_queries_of_empty_sequences(kvf, dtype, D, queries, beside):
+    """Sequences without any slot, alone or beside others: every row is written."""
+    H, G = 2, 4
+    lens = [(0, 0), (0, 0)] + ([beside] if beside else [])
+    w = World(kvf, lens, H, D, dtype, 16, seed=queries)
+    if beside:
+        w.step(H * G)
+    counts = [queries, queries + 1] + ([beside[1]] if beside else [])
+    b = w.cache.batch(w.seqs, counts, H * G)
+    q = _randn((sum(counts), H * G, D), dtype, 3)
+    out, lse = _attend_into(w, b, q, math.nan)
+    empty = 2 * queries + 1
+    assert (out[:empty] == 0).all() and (lse[:empty] == -math.inf).all()
+    if beside:
+        o, z, _, to, tz, _ = reference(w.k[2], w.v[2], q[empty:], D ** -0.5, 0, 0, dtype)
+        close(out[empty:], o, to)
+        close(lse[empty:], z, tz)
