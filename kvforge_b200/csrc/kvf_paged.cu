@@ -427,10 +427,10 @@ cudaError_t launch_paged_evict(const int* tables, const int* tables_dev, size_t 
   if (!tables_dev) std::copy(tables, tables + n + n * stride + n * new_stride, tab.v);
   // as many keys as shared memory holds
   constexpr size_t kKeyMost = 50 * 1024;
-  const size_t cached = std::min(longest, kKeyMost), smem = (cached + cached / 32 + 1) * 4;
-  cudaError_t e = cudaSuccess;
-  if (smem > kSmemOptIn - sizeof(int) * kSelBins)
-    e = cudaFuncSetAttribute(k_paged_select, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto key_bytes = [](size_t keys) { return (keys + keys / 32 + 1) * 4; };
+  const size_t cached = std::min(longest, kKeyMost), smem = key_bytes(cached);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, k_paged_select, key_bytes(kKeyMost));
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)c.heads, (unsigned)n, (unsigned)layers);
   k_paged_select<<<grid, kSelThreads, smem, st>>>(tab, c, (int)budget, (int)recent, (int)sinks, (int)cached, kept);

@@ -138,7 +138,8 @@ cudaError_t launch_paged_evict(const int* tables, const int* tables_dev, size_t 
                                size_t longest, const PagedLayer& c, size_t layers, size_t budget, size_t recent,
                                size_t sinks, int* kept, cudaStream_t st);
 
-// CUDA-core attention: every type and head_dim up to 256
+// CUDA-core attention: every type and head_dim up to kGenDimMost
+constexpr int kGenDimMost = 256;
 constexpr int kGenRows = 64, kGenRowsShort = 16, kGenKeys = 64;
 // tiles for more than kGenRows rows, head_dim up to kGenDimLong
 constexpr int kGenRowsLong = 128, kGenKeysLong = 128, kGenDimLong = 128;
@@ -174,8 +175,9 @@ cudaError_t launch_paged_chunk_weights(const PagedAttn& a, const PagedWork& w, s
                                        float decay, cudaStream_t st);
 
 #ifdef __CUDACC__
-// Opts a kernel in to `bytes` of dynamic shared memory, once per device (each
-// call site passes flags of its own; the same whichever thread sets them).
+// Opts a kernel in to `bytes` of dynamic shared memory, the most that any of its
+// launches asks for, once per device (each call site passes flags of its own). A
+// limit set for each launch could be lowered by another thread in front of it.
 struct OptInOnce {
   static constexpr int kDevices = 64;
   std::atomic<size_t> bytes[kDevices];

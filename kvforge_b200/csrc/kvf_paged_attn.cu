@@ -661,12 +661,6 @@ __global__ void __launch_bounds__(kGenThreads) k_paged_weights(PagedAttn a, cons
   }
 }
 
-template <typename K>
-cudaError_t opt_in(K kern, size_t smem) {
-  if (smem <= kSmemOptIn) return cudaSuccess;
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-}
-
 // rows may be read 16 bytes at a time
 template <typename T>
 bool wide_rows(const PagedAttn& a) {
@@ -680,9 +674,11 @@ bool wide_query(const PagedAttn& a) {
 template <typename T, int RT, int NU>
 cudaError_t attn_launch(const PagedAttn& a, const PagedWork& w, cudaStream_t st) {
   const int DP = (a.c.dim + 31) / 32 * 32;
-  const size_t smem = ((size_t)(16 * RT + 2 * kGenKeys) * DP + 16 * RT * kPStride) * sizeof(float);
+  auto bytes = [](size_t dp) { return ((16 * RT + 2 * kGenKeys) * dp + 16 * RT * kPStride) * sizeof(float); };
+  const size_t smem = bytes(DP);
   auto kern = k_paged_attn<T, RT, NU>;
-  cudaError_t e = opt_in(kern, smem);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, bytes(64 * NU));
   if (e != cudaSuccess) return e;
   kern<<<w.ctas, kGenThreads, smem, st>>>(a, w.segs, w.first, DP, wide_rows<T>(a), wide_query<T>(a));
   note_launches(1);
@@ -724,9 +720,11 @@ cudaError_t join_typed(const PagedAttn& a, const PagedWork& w, cudaStream_t st) 
 template <typename T, int RT>
 cudaError_t weights_launch(const PagedAttn& a, const PagedSlots* tiles, size_t ntiles, float decay, cudaStream_t st) {
   const int DP = (a.c.dim + 31) / 32 * 32;
-  const size_t smem = (size_t)(16 * RT + kGenKeys) * DP * sizeof(float);
+  auto bytes = [](size_t dp) { return (16 * RT + kGenKeys) * dp * sizeof(float); };
+  const size_t smem = bytes(DP);
   auto kern = k_paged_weights<T, RT>;
-  cudaError_t e = opt_in(kern, smem);
+  static OptInOnce done;
+  cudaError_t e = opt_in_once(done, kern, bytes(kGenDimMost));
   if (e != cudaSuccess) return e;
   kern<<<dim3((unsigned)ntiles, (unsigned)a.c.heads), kGenThreads, smem, st>>>(a, tiles, decay, DP, wide_rows<T>(a),
                                                                               wide_query<T>(a));

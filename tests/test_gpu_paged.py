@@ -1011,3 +1011,46 @@ def test_queries_of_empty_sequences(kvf, dtype, D, queries, beside):
         o, z, _, to, tz, _ = reference(w.k[2], w.v[2], q[empty:], D ** -0.5, 0, 0, dtype)
         close(out[empty:], o, to)
         close(lse[empty:], z, tz)
+
+
+def test_two_host_threads(kvf):
+    """Two caches, each with a thread and a stream of its own, whose calls launch
+    the same kernels with different amounts of shared memory."""
+    import threading
+    from kvforge_b200 import _lib as L
+    lib, ctx, caches, fail = L.lib(), L.context(0), [], []
+    for n, D in ((9000, 136), (30000, 256)):
+        w = World(kvf, [(n, 0), (3, 1)], 1, D, F32, 128, seed=D)
+        w.cache.weights.fill_(1.0)
+        caches.append(w)
+    torch.cuda.synchronize()
+    go = threading.Barrier(2)
+
+    def work(w):
+        c = w.cache
+        with torch.cuda.stream(torch.cuda.Stream()):
+            b = c.extend(w.seqs[1:], [1], 2)
+            q = torch.ones((1, 2, w.D), device="cuda")
+            out, kept = torch.empty_like(q), torch.empty(50, dtype=torch.int32, device="cuda")
+            st = torch.cuda.current_stream().cuda_stream
+            pool, scale = C.byref(c._pool), C.c_float(1.0)
+            pages = np.array(c.pages(w.seqs[0]), np.int32)
+            lens, new = np.array([w.lens[0][0]], np.int32), np.array(c._free[:1], np.int32)
+            go.wait()
+            for i in range(20000):
+                r = lib.kvf_paged_attention(ctx, b._h, pool, 0, q.data_ptr(), 2 * w.D, w.D, scale, 0.0, out.data_ptr(),
+                                            None, st)
+                if r == 0 and i % 20 == 0:
+                    r = lib.kvf_paged_evict(ctx, pool, 1, lens.ctypes.data, pages.ctypes.data, len(pages), 50, 0, 0,
+                                            new.ctypes.data, 1, kept.data_ptr(), st)
+                if r:
+                    fail.append((i, lib.kvf_last_error()))
+                    return
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in caches]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not fail, fail
