@@ -62,8 +62,9 @@ class PagedBatch:
     made once, used for every layer. tokens: new tokens of all sequences, one
     after another; starts: the first token of each sequence, and their number."""
 
-    def __init__(self, handle, seqs, states, query_heads: int, starts: np.ndarray):
+    def __init__(self, handle, owner, seqs, states, query_heads: int, starts: np.ndarray):
         self._h = handle
+        self._owner = owner  # what its cache is told by (not the cache: a batch keeps no pages)
         self._states = states  # (sequence, its page list) as the plan saw them
         self.seqs = seqs
         self.query_heads = query_heads
@@ -120,6 +121,7 @@ class PagedKVCache:
         self._scale = 1.0 / math.sqrt(self.head_dim)
         self._free = list(range(self.num_pages - 1, -1, -1))  # the lowest page is handed out first
         self._seqs = {}
+        self._self = object()
         self._next = 0
         self._last = torch.cuda.current_stream(self._dev)
         self._last_raw = self._last.cuda_stream
@@ -233,7 +235,7 @@ class PagedKVCache:
         h = self._plan(states, q, query_heads, window, sinks)
         starts = np.zeros(len(q) + 1, np.int64)
         np.cumsum(q, out=starts[1:])
-        return PagedBatch(h, seqs, states, int(query_heads), starts)
+        return PagedBatch(h, self._self, seqs, states, int(query_heads), starts)
 
     def _plan(self, states, q, query_heads, window, sinks) -> C.c_void_p:
         kv, _ = _ints([[s.length for s in states]])
@@ -256,6 +258,8 @@ class PagedKVCache:
         return raw
 
     def _handle(self, batch: PagedBatch):
+        if batch._owner is not self._self:
+            raise KvForgeError(L.ERR_INVALID_CONFIG, "the batch belongs to another cache")
         for s in batch._states:
             if not s.alive:
                 raise KvForgeError(L.ERR_INVALID_CONFIG, "a sequence of the batch was freed or evicted")

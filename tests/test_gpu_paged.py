@@ -1054,3 +1054,17 @@ def test_two_host_threads(kvf):
         t.join()
     torch.cuda.synchronize()
     assert not fail, fail
+
+
+def test_batch_of_another_cache(kvf):
+    """A batch names pages of its own cache: another one of the same shape refuses it."""
+    a, b = (kvf.PagedKVCache(8, 2, 64, page_size=16) for _ in range(2))
+    batch = a.extend([a.add()], [3], 4)
+    b.extend([b.add()], [3], 4)
+    k, q = _randn((3, 2, 64), F16, 1), _randn((3, 4, 64), F16, 2)
+    for call in (lambda: b.append(batch, k, k), lambda: b.attend(batch, q), lambda: b.attend(batch, q, decay=0.0)):
+        with pytest.raises(kvf.KvForgeError, match="another cache"):
+            call()
+    assert not b.keys.any() and not b.values.any() and not b.weights.any()
+    a.append(batch, k, k)
+    assert torch.isfinite(a.attend(batch, q)).all()
