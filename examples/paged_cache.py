@@ -58,6 +58,7 @@ def main():
             kept = cache.evict(over, args.budget, recent=RECENT, sinks=SINKS).kept
             print(f"evicted to {args.budget} tokens; layer 0, head 0 keeps {kept[0, 0, 0, :8].tolist()} ...")
         out = step(cache, [a, b], [1, 1], args.layers, gen)
+    cache.sync()  # raises if a kernel gave up
     print(f"answers: {cache.length(a)} and {cache.length(b)} tokens, output {tuple(out.shape)}")
 
     # a finished sequence goes to the archive, layer by layer, and its pages are free again

@@ -468,10 +468,12 @@ kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t lay
  * that has new tokens gets weight = decay * weight + sum over the new tokens
  * and the KV head's query heads of the slot's softmax weight (decay 0
  * overwrites). The sums run in a fixed order: results do not change from run
- * to run. Stream-ordered; no host synchronisation. A plan's first call with
- * decay >= 0 allocates device memory for the weights, which the plan keeps: make
- * one such call, with or without lse, before a stream capture of others
- * (KVF_ERR_PIPELINE inside one). */
+ * to run. Stream-ordered; no host synchronisation: a kernel that gives up a
+ * bounded wait leaves its outputs unfinished, and kvf_sync (or the next call that
+ * reads the context's status word) reports KVF_ERR_DEVICE_TIMEOUT. A plan's first
+ * call with decay >= 0 allocates device memory for the weights, which the plan
+ * keeps: make one such call, with or without lse, before a stream capture of
+ * others (KVF_ERR_PIPELINE inside one). */
 kvf_status kvf_paged_attention(kvf_ctx* ctx, const kvf_paged_plan* plan, const kvf_paged_pool* pool, size_t layer,
                                const void* query, size_t q_token_stride, size_t q_head_stride, float scale,
                                float decay, void* out, float* lse, void* stream);

@@ -280,6 +280,14 @@ class PagedKVCache:
             raise KvForgeError(L.ERR_SHAPE_MISMATCH, f"layer {layer} of {self.num_layers}")
         return layer
 
+    def sync(self) -> None:
+        """Waits for the cache's calls so far, and raises KvForgeError when a
+        kernel of theirs gave up a bounded wait (KVF_ERR_DEVICE_TIMEOUT: what it was
+        to write is unfinished) or when one of the codec's reported an error: the
+        device has one status word, which the first call that reads it clears.
+        Nothing else here waits for the GPU or looks."""
+        L.check(self._lib.kvf_sync(self._ctx, self._enter()))
+
     # ---- operators ----------------------------------------------------------------
     def append(self, batch: PagedBatch, keys: torch.Tensor, values: torch.Tensor, layer: int = 0) -> None:
         """Writes the batch's new tokens, keys and values [tokens, num_heads,

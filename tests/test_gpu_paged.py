@@ -1068,3 +1068,21 @@ def test_batch_of_another_cache(kvf):
     assert not b.keys.any() and not b.values.any() and not b.weights.any()
     a.append(batch, k, k)
     assert torch.isfinite(a.attend(batch, q)).all()
+
+
+def test_a_wait_that_gave_up_is_told(kvf):
+    """A bounded device wait that runs out (the library's self-test of one) is told
+    by sync, once, and the cache goes on."""
+    from kvforge_b200 import _lib as L
+    w = World(kvf, [(40, 1), (7, 30)], 2, 64, F16, 16, seed=31)
+    q = w.step(4)
+    w.cache.sync()
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    L.check(L.lib().kvf_selftest_wait_timeout(L.context(0), L.WAIT_MBARRIER, st))
+    w.cache.attend(w.batch, q)
+    with pytest.raises(kvf.KvForgeError) as e:
+        w.cache.sync()
+    assert e.value.status == L.ERR_DEVICE_TIMEOUT
+    w.cache.sync()
+    check(w, q, decay=0.0)
+    w.cache.sync()
