@@ -496,6 +496,13 @@ __global__ void __launch_bounds__(kWeightThreads) k_paged_decode_weights(PagedAt
       for (int r = 0; r < 8; ++r) {
         if (r0 + r >= rows) continue;
         const float z = lse2[hs][r0 + r];
+        if (z != z) {  // a NaN row: NaN for the slots that it sees, nothing for the others
+          const int pos = n - nq + (r0 + r) / a.group;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (paged_sees(pos, j + e, a.window, a.sinks)) t[e] = z;
+          continue;
+        }
         t[0] += exp2f(x[r].x - z);
         t[1] += exp2f(x[r].y - z);
         t[2] += exp2f(x[r].z - z);

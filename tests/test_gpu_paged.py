@@ -1086,3 +1086,25 @@ def test_a_wait_that_gave_up_is_told(kvf):
     w.cache.sync()
     check(w, q, decay=0.0)
     w.cache.sync()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens,row", [((100, 4), 1), ((500, 7), 0), ((3, 2), 0), ((200, 60), 20)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 2), (70, 0)])
+def test_weights_of_a_nan_row(kvf, dtype, lens, row, window, sinks):
+    """A query of NaN gives NaN weights to the slots that it sees, and to no others."""
+    H, G, D = 2, 2, 64
+    w = World(kvf, [lens], H, D, dtype, 16, seed=40)
+    q = w.step(H * G, window, sinks)
+    bad = q.clone()
+    bad[row, 1] = math.nan  # KV head 0
+    w.cache.attend(w.batch, bad, decay=0.0)
+    (a, c), n = lens, sum(lens)
+    pages = torch.tensor(w.cache.pages(w.seqs[0]), device="cuda")
+    got = w.cache.weights[0, pages].transpose(0, 1).reshape(H, -1)[:, :n]
+    _, _, want, _, _, tol = reference(w.k[0], w.v[0], q, D ** -0.5, window, sinks, dtype)
+    see = seen(n, c, window, sinks)[row]
+    s = (w.k[0][:, 0].double() @ q[row, 1].double() * D ** -0.5).masked_fill(~see, -math.inf)
+    want[0] -= torch.softmax(s, 0)
+    want[0, see] = math.nan
+    close(got, want, tol + 2.0 ** -40)
