@@ -337,12 +337,13 @@ class PagedKVCache:
             raise KvForgeError(L.ERR_INVALID_CONFIG, "budget must be at least 1 and hold the sinks and recent tokens")
         states = [self._seqs[s] for s in seqs]
         lens = [min(budget, s.length) for s in states]
+        # (first: where memory runs out, no page has been taken)
+        kept = self.weights.new_empty((self.num_layers, len(seqs), self.num_heads, budget), dtype=torch.int32)
         taken = self._take(sum(self._pages_for(n) for n in lens))
         lists, at = [], 0
         for n in lens:
             lists.append(taken[at:at + self._pages_for(n)])
             at += len(lists[-1])
-        kept = self.weights.new_empty((self.num_layers, len(seqs), self.num_heads, budget), dtype=torch.int32)
         try:
             kv, _ = _ints([[s.length for s in states]])
             table, stride = _ints([s.pages for s in states])

@@ -1108,3 +1108,15 @@ def test_weights_of_a_nan_row(kvf, dtype, lens, row, window, sinks):
     want[0] -= torch.softmax(s, 0)
     want[0, see] = math.nan
     close(got, want, tol + 2.0 ** -40)
+
+
+def test_evict_without_memory_for_its_result(kvf):
+    """A budget whose list of kept slots (2^48 bytes) fits nowhere: an error, and no page is lost."""
+    cache = kvf.PagedKVCache(8, 16, 8, page_size=16, num_layers=4096)
+    s = cache.add(40)
+    free = cache.free_pages
+    with pytest.raises(RuntimeError):
+        cache.evict([s], 2 ** 30)
+    assert cache.free_pages == free and cache.length(s) == 40
+    cache.evict([s], 20)
+    assert cache.free_pages == free + 1 and cache.length(s) == 20
