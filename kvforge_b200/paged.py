@@ -241,9 +241,11 @@ class PagedKVCache:
         kv, _ = _ints([[s.length for s in states]])
         ql, _ = _ints([q])
         table, stride = _ints([s.pages for s in states])
+        # ctypes cuts whole numbers to 32 bits: longer ones than any sequence mean the same as 2^31 - 1
+        window, sinks = (max(-1, min(int(x), 2 ** 31 - 1)) for x in (window, sinks))
         h = C.c_void_p()
         L.check(self._lib.kvf_paged_plan_create(self._ctx, self._pool_ref, len(states), ql, kv, table, stride,
-                                                int(query_heads), int(window), int(sinks), C.byref(h), self._enter()))
+                                                int(query_heads), window, sinks, C.byref(h), self._enter()))
         return h
 
     def _enter(self) -> int:

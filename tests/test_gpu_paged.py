@@ -1120,3 +1120,13 @@ def test_evict_without_memory_for_its_result(kvf):
     assert cache.free_pages == free and cache.length(s) == 40
     cache.evict([s], 20)
     assert cache.free_pages == free + 1 and cache.length(s) == 20
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 31, 0), (2 ** 32 + 5, 0), (2 ** 70, 3), (7, 2 ** 32), (7, 2 ** 32 + 3)])
+def test_windows_beyond_32_bits(kvf, window, sinks):
+    """A window, or sinks, longer than any sequence hides nothing."""
+    w = World(kvf, [(300, 1), (50, 70)], 2, 64, F16, 16, seed=41)
+    check(w, w.step(4, window, sinks), decay=0.0)
+    for bad in (dict(window=-2 ** 32), dict(window=9, sinks=-2 ** 32)):
+        with pytest.raises(kvf.KvForgeError):
+            w.cache.batch(w.seqs, [1, 1], 4, **bad)
