@@ -314,8 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(32 * (w & 3)) << 16;
     const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * DP;
     const int D = a.c.dim;
-    // a negative scale turns the queries' sign, a zero one makes them zero
-    const float c = a.scale2 == 0.0f ? 1.0f : fabsf(a.scale2), lag = 8.0f / c;
+    // a negative scale turns the queries' sign; the smallest number stands for zero
+    // (every finite score becomes 0 to within 5e-7, and NaN stays NaN)
+    const float c = a.scale2 == 0.0f ? 1.4e-45f : fabsf(a.scale2), lag = 8.0f / c;
     int cnt_s = 0, cnt_o = 0;
     uint32_t turns = 0;
     int ring0 = 0;  // tiles of K and V before this segment
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool two = s.tiles() == kTiles;
       float m = -INFINITY, l = 0.0f;
       if (count > 0) {
-        const uint32_t q_xor = a.scale2 < 0.0f ? 0x80008000u : 0u, q_and = a.scale2 == 0.0f ? 0u : 0xFFFFFFFFu;
+        const uint32_t q_xor = a.scale2 < 0.0f ? 0x80008000u : 0u;
         const uint16_t* p =
             static_cast<const uint16_t*>(a.q) + (size_t)(s.q0 + tok) * a.q_token + (size_t)hq * a.q_head;
 #pragma unroll
@@ -347,10 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                              e[4] | ((uint32_t)e[5] << 16), e[6] | ((uint32_t)e[7] << 16));
             }
           }
-          x.x = (x.x & q_and) ^ q_xor;
-          x.y = (x.y & q_and) ^ q_xor;
-          x.z = (x.z & q_and) ^ q_xor;
-          x.w = (x.w & q_and) ^ q_xor;
+          x.x ^= q_xor;
+          x.y ^= q_xor;
+          x.z ^= q_xor;
+          x.w ^= q_xor;
           *reinterpret_cast<uint4*>(sm + i * kBytes + tile_off(t, ch)) = x;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

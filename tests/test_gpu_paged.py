@@ -1130,3 +1130,21 @@ def test_windows_beyond_32_bits(kvf, window, sinks):
     for bad in (dict(window=-2 ** 32), dict(window=9, sinks=-2 ** 32)):
         with pytest.raises(kvf.KvForgeError):
             w.cache.batch(w.seqs, [1, 1], 4, **bad)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 0.3, -0.3])
+def test_nan_queries_at_any_scale(kvf, dtype, scale):
+    """A NaN query gives NaN, also where the scale is 0; the other rows are as ever."""
+    w = World(kvf, [(300, 1), (50, 70), (9, 3)], 2, 64, dtype, 32, seed=42, big=30.0)
+    for i in range(3):
+        w.cache.append(w.cache.batch(w.seqs[i:i + 1], [w.lens[i][0]]), w.k[i][:w.lens[i][0]], w.v[i][:w.lens[i][0]])
+    q = w.step(8) * 30
+    want, want_lse = check(w, q, scale=scale)
+    bad = q.clone()
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for t, h in ((0, 3), (5, 0), (40, 7), (72, 2)):
+        bad[t, h, 11], hit[t, h] = math.nan, True
+    out, lse = w.cache.attend(w.batch, bad, scale=scale, return_lse=True)
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
