@@ -375,14 +375,14 @@ kvf_status check_shape(size_t H, size_t T, size_t D) {
   return KVF_OK;
 }
 
-// a reader of `c` (a compressed layer, a paged plan) on stream `st`: waits for
-// the object's buffers to be complete when `st` is not the stream that built them
-template <class Obj>
-kvf_status reader_enter(const Obj* c, cudaStream_t st) {
+// a reader of `c` on stream `st`: waits for the object's buffers to be
+// complete when `st` is not the stream that built them
+kvf_status reader_enter(const kvf_compressed* c, cudaStream_t st) {
   if (c->ready && st != c->stream) KVF_CUDA(cudaStreamWaitEvent(st, c->ready, 0));
   return KVF_OK;
 }
-// ... and after its last use: records on `st` what the object's free waits for
+// ... and after its last use (of a paged plan, too): records on `st` what the
+// object's free waits for
 template <class Obj>
 kvf_status reader_leave(const Obj* c, cudaStream_t st) {
   if (st == c->stream) return KVF_OK;
@@ -1258,7 +1258,6 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
   p->seqs.stride = max_pages;
   p->seqs.kv_len = reinterpret_cast<const int*>(d + at_kv);
   p->seqs.q_start = reinterpret_cast<const int*>(d + at_q);
-  p->seqs.n = (int)n;
   for (size_t i = 0; i < hosts.size(); ++i) {
     const PagedWorkHost& h = hosts[i];
     PagedWork w;
@@ -1266,7 +1265,6 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     w.row_tile = h.row_tile;
     w.key_tile = h.key_tile;
     w.ctas = (int)h.first.size() - 1;
-    w.segs_n = (int)h.segs.size();
     w.joins_n = (int)h.joins.size();
     w.parts = h.parts;
     w.segs = reinterpret_cast<const PagedSeg*>(d + at[i].segs);

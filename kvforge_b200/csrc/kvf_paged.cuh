@@ -26,7 +26,6 @@ struct PagedSeqs {
   size_t stride = 0;
   const int* kv_len = nullptr;   // [n]
   const int* q_start = nullptr;  // [n + 1] first token of each sequence
-  int n = 0;
 };
 
 // Attention work. A KV head's query rows of one sequence are numbered
@@ -50,7 +49,7 @@ enum PagedKernel { kPagedGeneric = 0, kPagedDecode = 1, kPagedChunk = 2 };
 struct PagedWork {
   int kernel = kPagedGeneric;
   int row_tile = 0, key_tile = 0;
-  int ctas = 0, segs_n = 0, joins_n = 0, parts = 0;
+  int ctas = 0, joins_n = 0, parts = 0;
   const PagedSeg* segs = nullptr;  // device
   const int* first = nullptr;
   const PagedJoin* joins = nullptr;

@@ -37,7 +37,6 @@
 // TMEM: 2 x 128 columns of scores (numerators over them), 2 x D of sums. Every
 // wait is bounded; one that runs out ends all roles and sets kDevErrTimeout.
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 
 #include "kvf_paged_tc.cuh"
