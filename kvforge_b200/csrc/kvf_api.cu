@@ -1199,7 +1199,8 @@ kvf_status paged_plan_body(kvf_paged_plan* p, size_t n, const int32_t* q_lens, c
     } else {
       add(kPagedGeneric, 1, few, kGenRowsShort, kGenKeys, 3 * sms, 2, 1);
       // Sequences of more than kGenRows rows: a tile of 128 x 128 takes an SM 2.75
-      // times as long as one of 64 x 64 (35 and 12.7 us at head_dim 128), and there
+      // times as long as one of 64 x 64 (35 and 12.7 us at head_dim 128, the only
+      // one where the ratio was measured), and there
       // are four of those to one, or fewer in narrow windows: eight chunks of 392
       // tokens, 128 query heads, window of 2: 1026 us with large tiles, 830 with
       // small ones; of 100: 1657 and 1641; of 1000: 4230 and 5300

@@ -7,8 +7,12 @@
 //   O' = f O + sum 2^(s2 - m') v
 // and out = O / l, lse = (m + log2 l) ln 2. A segment of the slots leaves
 // (m, l, O); k_paged_join adds segments up with the weights 2^(m_i - max m).
-// These kernels serve f32 pools, whose products need all 24 bits, and head
-// dims that the tensor-core kernels do not take.
+// These kernels serve f32 pools and head dims that the tensor-core kernels do
+// not take: products of all 24 bits on the multiply-add units. (Operands split
+// into parts would give f32 products on the tensor cores too; not built.)
+// Whole calls, against the bytes' time in brackets: f32 single tokens of 16
+// sequences of 3000 to 16000 slots, 8 KV and 64 query heads of 128, 799 us (178);
+// the same in bf16 with 32 query heads of 256, 2464 (178).
 #include <cfloat>
 #include <cmath>
 

@@ -6,8 +6,10 @@
 // exponentials; at D = 128 an SM's tensor core needs 1024 cycles for a tile of
 // 128 rows by 128 slots, and its 16 exponentials per cycle need 1024 as well,
 // so the kernel is bound by both and must keep them busy at the same time.
-// 2048 tokens on 30720 cached, 32 query and 8 KV heads of 128 in f16: 955-990
-// us, 1080-1120 TFLOP/s, the tensor core busy 60 % of the cycles.
+// 2048 tokens on 30720 cached, 32 query and 8 KV heads of 128 in f16: 957-967
+// us at 1965 MHz (1100 TFLOP/s), 1110-1140 in steady calls, whose load brings
+// the clock down. Neither unit is full (45 % each in ncu, 1184 tokens on 8192): a
+// row tile's products wait for its softmax and the other way round.
 //
 // One persistent CTA per SM walks segments of (sequence, KV head, 256 rows),
 // two row tiles of 128 whose work alternates on the tensor core: while one
@@ -21,7 +23,7 @@
 //     turns: left to themselves they fall into step, both in the softmax and
 //     then both on the tensor core (4400 instead of 3400 cycles per pair of
 //     tiles). Eight more warps, two threads a row, are slower (993 against 960
-//     us): the halves of a row have to meet for its maximum.
+//     us at full clock): the halves of a row have to meet for its maximum.
 //   warp 8: tensor-map loads of K and V tiles, a box per page.
 //   warps 9, 10: the MMAs of row tile 0 and 1, each issued by one thread, so
 //     that one warp's waits (about 110 cycles even when there is nothing to
