@@ -39,6 +39,7 @@
 // TMEM: 2 x 128 columns of scores (numerators over them), 2 x D of sums. Every
 // wait is bounded; one that runs out ends all roles and sets kDevErrTimeout.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "kvf_paged_tc.cuh"
@@ -317,7 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int D = a.c.dim;
     // a negative scale turns the queries' sign; the smallest number stands for zero
     // (every finite score becomes 0 to within 5e-7, and NaN stays NaN)
-    const float c = a.scale2 == 0.0f ? 1.4e-45f : fabsf(a.scale2), lag = 8.0f / c;
+    const float c = a.scale2 == 0.0f ? 1.4e-45f : fabsf(a.scale2);
+    const float lag = fminf(8.0f / c, FLT_MAX);  // finite: nothing seen yet (-inf) stays -inf with it added
     int cnt_s = 0, cnt_o = 0;
     uint32_t turns = 0;
     int ring0 = 0;  // tiles of K and V before this segment

@@ -1148,3 +1148,14 @@ def test_nan_queries_at_any_scale(kvf, dtype, scale):
     out, lse = w.cache.attend(w.batch, bad, scale=scale, return_lse=True)
     assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
     assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale", [0.0, 1e-44, -1e-40, 1e-38, 1e-30])
+def test_vanishing_scales_under_a_window(kvf, dtype, scale):
+    """Rows whose first tiles are all masked, at scales that make every score the same."""
+    w = World(kvf, [(152, 237), (600, 300), (90, 2)], 2, 64, dtype, 32, seed=43)
+    check(w, w.step(2, 1, 0), 1, 0, scale=scale, decay=0.0)
+    b = w.cache.batch(w.seqs, [c for _, c in w.lens], 2, 41, 3)
+    w.batch = b
+    check(w, _randn((b.tokens, 2, 64), dtype, 9), 41, 3, scale=scale, decay=0.0)
