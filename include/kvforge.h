@@ -461,7 +461,8 @@ kvf_status kvf_paged_gather(kvf_ctx* ctx, const kvf_paged_pool* pool, size_t lay
  * head_dim] contiguous, of the pool's dtype; lse (or NULL) f32 [tokens,
  * query_heads], the natural logarithm of the softmax's sum. Scores, softmax
  * and sums are held in f32; with f16 and bf16 pools the softmax's numerators
- * are rounded to that type for the product with the values. A row that sees
+ * are rounded to that type for the product with the values (with f16 those below
+ * 2^-25 become 0, and an infinite value so weighted may give NaN). A row that sees
  * nothing, or only scores of -inf, gives out 0 and lse -inf. Slots that no row
  * sees may hold anything, NaN included.
  * decay < 0 leaves the weights alone; otherwise every slot of every sequence
